@@ -255,6 +255,82 @@ int mq_debug_set_error(int device, unsigned flags);
  * only after a launch reported a watchdog error. Synchronous. */
 int mq_reset_workspace(int device);
 
+/* ---- A paged K/V cache, for batches of sequences that share rows. No counterpart in the reference
+ * (one contiguous cache a decoder, csrc/megakernel/megakernel_decode.py:140-146).
+ *
+ * A pool of pages, in device memory: k and v [num_layers, num_pages, num_kv_heads, page_size,
+ * head_dim], contiguous, 16-bit values (dtype), 16-byte aligned; bounds (may be NULL where an entry
+ * does not need them) [num_layers, num_pages, num_kv_heads, 2, head_dim], the least and the greatest
+ * key entry of each dim over a page's filled rows. page_size is 16, 32, 64, 128 or 256, head_dim 64
+ * or 128. A page id stands for that page of every layer.
+ *
+ * A table holds the page ids of one sequence in order: its position i is row i % page_size of page
+ * table[i / page_size]. Entries that no position needs are never read. Tables and lens are device
+ * int32; ids in them that are outside the pool read nothing from it: the outputs of a sequence that
+ * needs such a page are not numbers, an appended row is dropped.
+ *
+ * Nothing here uses the library workspace: calls on several streams may overlap as long as no page
+ * that one writes is used by another. Every entry is stream-ordered, allocates nothing and can be
+ * captured; page ids given as HOST arrays are copied during the call. */
+#define MQ_BF16 0
+#define MQ_FP16 1
+#define MQ_MAX_TABLE_WIDTH 8192
+typedef struct MqPagePool {
+  void* k;
+  void* v;
+  void* bounds;
+  int num_layers, num_pages, num_kv_heads, page_size, head_dim, dtype;
+} MqPagePool;
+
+/* Copies pages src[i] to dst[i] (HOST arrays) of every layer: K, V and, where given, bounds. The dst
+ * must differ from each other and from every src. */
+int mq_pages_copy(const MqPagePool* pool, const int* src, const int* dst, int n, hipStream_t stream);
+
+/* Positions 0 .. length - 1 of a contiguous cache [num_layers, num_kv_heads, max_seq_len, head_dim]
+ * into the pages of the HOST list (ceil(length / page_size) of them), and their bounds where the
+ * pool has them; and back. Rows of the last page behind `length` stay as they are. */
+int mq_pages_load(const MqPagePool* pool, const int* pages, int length, const void* k_cache, const void* v_cache,
+                  int max_seq_len, hipStream_t stream);
+int mq_pages_store(const MqPagePool* pool, const int* pages, int length, void* k_cache, void* v_cache,
+                   int max_seq_len, hipStream_t stream);
+
+/* One new K and V row a sequence, k and v [batch, num_kv_heads, head_dim] with strides in elements
+ * (multiples of 8; the last is 1), to position lens[b] of sequence b (lens is not changed), and the
+ * page's bounds where the pool has them. One layer (num_layers 1). tables [batch, width] with a row
+ * stride; no two sequences may append to one page. */
+int mq_pages_append(const MqPagePool* pool, const void* k, const void* v, long long k_sb, long long k_sh,
+                    long long v_sb, long long v_sh, const int* tables, long long table_stride, int width,
+                    const int* lens, int batch, hipStream_t stream);
+
+/* Bytes of workspace of one call of the attentions below: prefix_len, max_len and num_q_heads as
+ * given to it; top 0 for mq_shared_prefix_attention. For mq_sparse_attention prefix_len is 0 and
+ * max_len min(top, width) * page_size. */
+int mq_attention_workspace(const MqPagePool* pool, int num_q_heads, int batch, int prefix_len, int max_len, int top,
+                           size_t* bytes);
+
+/* Attention of one query token a sequence, q and out [batch, num_q_heads, head_dim] with strides in
+ * elements (multiples of 8; the last is 1), in the pool's type, over the prefix_len positions of the
+ * prefix, which all sequences share, and then over lens[b] positions of the sequence's own table
+ * (more than width * page_size count as that many): out = softmax(scale q K^T) V. Query head i reads
+ * kv head i / (num_q_heads / num_kv_heads). A sequence without any position gets zeros. One layer: k
+ * and v are its base addresses. max_len is only the length that the launch is laid out for (for
+ * instance the longest of lens): every value gives the same outputs but for the order of their
+ * sums; 0 asks for the prefix alone. */
+int mq_shared_prefix_attention(const MqPagePool* pool, const void* q, long long q_sb, long long q_sh, void* out,
+                               long long o_sb, long long o_sh, int num_q_heads, int batch, const int* prefix_pages,
+                               int prefix_len, const int* tables, long long table_stride, int width, const int* lens,
+                               int max_len, float scale, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* Attention of one query token a sequence over `top` of its pages: its last one and the top - 1
+ * others with the largest scores, all pages if it has no more. The score of a page for a kv head is
+ * the sum, over that head's query heads and the dims, of max(q lo, q hi) with the page's bounds lo
+ * and hi, in 64 bits; of equal scores the lower position wins. chosen int32 [batch, num_kv_heads,
+ * top]: their numbers in the table in ascending order, then -1. Everything else as above. */
+int mq_sparse_attention(const MqPagePool* pool, const void* q, long long q_sb, long long q_sh, void* out,
+                        long long o_sb, long long o_sh, int* chosen, int num_q_heads, int batch, const int* tables,
+                        long long table_stride, int width, const int* lens, int top, float scale, void* workspace,
+                        size_t workspace_bytes, hipStream_t stream);
+
 /* Human-readable name of a status code. */
 const char* mq_strerror(int status);
 

@@ -25,6 +25,11 @@ MQ_VARIANT_SPLIT = 2
 # rejects the rest)
 MAX_CONTEXT = 16384
 
+# types of a page pool and the widest page table (include/megaqwen_amd.h)
+MQ_BF16 = 0
+MQ_FP16 = 1
+MQ_MAX_TABLE_WIDTH = 8192
+
 LAYER_FIELDS = (
     "input_layernorm_weight",
     "q_proj_weight",
@@ -53,9 +58,20 @@ class MqDecodeStep(ctypes.Structure):
                 ("count", ctypes.c_int)]
 
 
+class MqPagePool(ctypes.Structure):
+    """Mirror of the C struct: a pool of K/V pages (include/megaqwen_amd.h)."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("bounds", ctypes.c_void_p)] + [
+        (name, ctypes.c_int) for name in ("num_layers", "num_pages", "num_kv_heads", "page_size", "head_dim", "dtype")]
+
+
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _f = ctypes.c_float
+_ll = ctypes.c_longlong
+_sz = ctypes.c_size_t
+_pool = ctypes.POINTER(MqPagePool)
+_ints = ctypes.POINTER(_i)
 
 # name -> argtypes; every entry returns int (MQ_OK or MQ_ERR_*) except mq_strerror.
 _DECODE_ARGS = [_i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
@@ -82,6 +98,20 @@ SIGNATURES = {
     "mq_set_launch_mode": [_i],
     "mq_debug_set_error": [_i, ctypes.c_uint],
     "mq_reset_workspace": [_i],
+    "mq_pages_copy": [_pool, _ints, _ints, _i, _vp],
+    # pool, pages (host), length, k cache, v cache, max_seq_len, stream
+    "mq_pages_load": [_pool, _ints, _i, _vp, _vp, _i, _vp],
+    "mq_pages_store": [_pool, _ints, _i, _vp, _vp, _i, _vp],
+    # pool, k, v, strides, tables, table stride, width, lens, batch, stream
+    "mq_pages_append": [_pool, _vp, _vp, _ll, _ll, _ll, _ll, _vp, _ll, _i, _vp, _i, _vp],
+    "mq_attention_workspace": [_pool, _i, _i, _i, _i, _i, ctypes.POINTER(_sz)],
+    # pool, q and strides, out and strides, query heads, batch, prefix pages, prefix length, tables, table
+    # stride, width, lens, max_len, scale, workspace, its bytes, stream
+    "mq_shared_prefix_attention": [_pool, _vp, _ll, _ll, _vp, _ll, _ll, _i, _i, _vp, _i, _vp, _ll, _i, _vp, _i, _f, _vp, _sz,
+                                   _vp],
+    # pool, q and strides, out and strides, chosen, query heads, batch, tables, table stride, width, lens,
+    # top, scale, workspace, its bytes, stream
+    "mq_sparse_attention": [_pool, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _i, _i, _vp, _ll, _i, _vp, _i, _f, _vp, _sz, _vp],
     "mq_strerror": [_i],
 }
 

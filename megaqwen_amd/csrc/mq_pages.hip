@@ -1,0 +1,950 @@
+// A paged K/V cache on MI355X (gfx950): moving pages, appending rows, and the attentions that
+// read it. The reference keeps one contiguous cache (csrc/megakernel/megakernel_decode.py:140-146)
+// and has no counterpart of these.
+//
+// A pool holds [layers, pages, kv heads, page size, head dim] of 16-bit values for K and as many for
+// V, so that one page of one layer is one contiguous run and one page's rows of one head are one
+// inside it: an attention workgroup reads whole runs of page size * head dim, and a fork or a
+// compaction moves a layer's page as a single run. Page ids hold for every layer. `bounds`
+// [layers, pages, kv heads, 2, head dim] are a page's least and greatest key entries.
+
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+#include <string.h>
+
+#include "megaqwen_amd.h"
+#include "mq_common.h"
+#include "mq_pages.h"
+
+namespace mq {
+namespace pg {
+
+// ------------------------------------------------------------------ moving pages
+// Page ids travel in the argument block, so that no copy from host memory waits for the device and a
+// captured launch keeps them: a block of 4 KB holds 448 pairs and the rest of the arguments; a small
+// one holds 32, which costs the host less to fill and send.
+constexpr int LIST_LONG = 448, LIST_SHORT = 32;
+
+template <int N>
+struct CopyArgs {
+  void* base[3];         // K, V, bounds (or null)
+  uint32_t page_bytes;   // one page of one layer of K or V
+  uint32_t bounds_bytes; // one page of one layer of the bounds
+  uint32_t per_page;     // workgroups a page of K or V
+  int num_pages, n;
+  int2 ids[N];           // (from, to)
+};
+
+constexpr int CT = 256;              // threads
+constexpr int CU = 4;                // 16-byte units a thread
+constexpr uint32_t CB = CT * CU * 16;  // bytes a workgroup
+
+// Workgroup (part of a page, pair, layer): a run of at most 16 KB of K or V, or the page's bounds.
+template <int N>
+__global__ void __launch_bounds__(CT) copy_kernel(CopyArgs<N> A) {
+  const uint32_t part = blockIdx.x, which = part < A.per_page ? 0 : part < 2 * A.per_page ? 1 : 2;
+  const uint32_t bytes = which == 2 ? A.bounds_bytes : A.page_bytes;
+  const uint32_t off = (which == 2 ? part - 2 * A.per_page : which ? part - A.per_page : part) * CB;
+  const int2 id = A.ids[blockIdx.y];
+  const size_t layer = (size_t)blockIdx.z * A.num_pages;
+  const char* src = static_cast<const char*>(A.base[which]) + (layer + id.x) * bytes;
+  char* dst = static_cast<char*>(A.base[which]) + (layer + id.y) * bytes;
+  u32x4 w[CU];
+#pragma unroll
+  for (int u = 0; u < CU; u++) {
+    const uint32_t o = off + 16 * (threadIdx.x + CT * u);
+    if (o < bytes) w[u] = __builtin_nontemporal_load((gu32x4*)(src + o));
+  }
+#pragma unroll
+  for (int u = 0; u < CU; u++) {
+    const uint32_t o = off + 16 * (threadIdx.x + CT * u);
+    if (o < bytes) __builtin_nontemporal_store(w[u], reinterpret_cast<u32x4*>(dst + o));
+  }
+}
+
+template <int N>
+struct MoveArgs {
+  uint16_t *k, *v, *bounds;  // the pool
+  uint16_t *kc, *vc;         // the contiguous cache [layers, kv heads, max_seq, head dim]
+  int num_pages, hkv, page, d, max_seq, first, length;  // first: position of the list's first page
+  int ids[N];
+};
+
+// the least (greatest) of two values; a value that is not a number wins, as in torch.amin
+__device__ __forceinline__ float least(float a, float x) { return x < a || x != x ? x : a; }
+__device__ __forceinline__ float greatest(float a, float x) { return x > a || x != x ? x : a; }
+
+template <bool F16>
+__device__ __forceinline__ float to_f32(uint32_t b) {
+  return F16 ? (float)__builtin_bit_cast(_Float16, (unsigned short)b) : bf2f(b & 0xffffu);
+}
+template <bool F16>
+__device__ __forceinline__ void to_f32x8(const u32x4 w, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    f[2 * i] = to_f32<F16>(w[i] & 0xffffu);
+    f[2 * i + 1] = to_f32<F16>(w[i] >> 16);
+  }
+}
+// values that came from 16 bits go back without rounding
+template <bool F16>
+__device__ __forceinline__ u32x4 from_f32x8(const float (&f)[8]) {
+  u32x4 w;
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    w[i] = F16 ? (uint32_t)__builtin_bit_cast(unsigned short, (_Float16)f[2 * i]) |
+                     (uint32_t)__builtin_bit_cast(unsigned short, (_Float16)f[2 * i + 1]) << 16
+               : pack_bf2(f[2 * i], f[2 * i + 1]);
+  return w;
+}
+
+// Workgroup (kv head, page, layer): the page's filled rows between the contiguous cache and the
+// pool, K and V, and on the way in the bounds of its keys. Thread t takes 8 dims of rows t / (d / 8),
+// ... in steps of CT / (d / 8) rows.
+template <int N, bool IN, bool F16>
+__global__ void __launch_bounds__(CT) move_kernel(MoveArgs<N> A) {
+  __shared__ float s_lo[CT][9], s_hi[CT][9];  // (9: a column of eight lanes' rows lies in distinct banks)
+  const int h = blockIdx.x, j = blockIdx.y, l = blockIdx.z, cpr = A.d / 8, c = threadIdx.x % cpr, step = CT / cpr;
+  const int first = A.first + j * A.page, rows = min(A.page, A.length - first);
+  const size_t in_pool = (((size_t)l * A.num_pages + A.ids[j]) * A.hkv + h) * A.page * A.d + 8 * c;
+  const size_t flat = (((size_t)l * A.hkv + h) * A.max_seq + first) * A.d + 8 * c;
+  float lo[8], hi[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) lo[i] = INFINITY, hi[i] = -INFINITY;
+  for (int r = threadIdx.x / cpr; r < rows; r += step) {
+    const size_t p = in_pool + (size_t)r * A.d, q = flat + (size_t)r * A.d;
+    const u32x4 kw = ldw(IN ? A.kc + q : A.k + p), vw = ldw(IN ? A.vc + q : A.v + p);
+    __builtin_nontemporal_store(kw, reinterpret_cast<u32x4*>(IN ? A.k + p : A.kc + q));
+    __builtin_nontemporal_store(vw, reinterpret_cast<u32x4*>(IN ? A.v + p : A.vc + q));
+    if (IN && A.bounds) {
+      float f[8];
+      to_f32x8<F16>(kw, f);
+#pragma unroll
+      for (int i = 0; i < 8; i++) lo[i] = least(lo[i], f[i]), hi[i] = greatest(hi[i], f[i]);
+    }
+  }
+  if (!IN || !A.bounds) return;
+#pragma unroll
+  for (int i = 0; i < 8; i++) s_lo[threadIdx.x][i] = lo[i], s_hi[threadIdx.x][i] = hi[i];
+  __syncthreads();
+  if ((int)threadIdx.x >= cpr) return;
+  for (int t = threadIdx.x + cpr; t < CT; t += cpr)
+#pragma unroll
+    for (int i = 0; i < 8; i++) lo[i] = least(lo[i], s_lo[t][i]), hi[i] = greatest(hi[i], s_hi[t][i]);
+  uint16_t* b = A.bounds + (((size_t)l * A.num_pages + A.ids[j]) * A.hkv + h) * 2 * A.d + 8 * c;
+  *reinterpret_cast<u32x4*>(b) = from_f32x8<F16>(lo);
+  *reinterpret_cast<u32x4*>(b + A.d) = from_f32x8<F16>(hi);
+}
+
+// Workgroup b: sequence b's new K and V row to its position lens[b], and the page's bounds: the row
+// itself where it is the page's first, the least and greatest with it otherwise. A position behind
+// the table or a page outside the pool: nothing is written.
+template <bool F16>
+__global__ void __launch_bounds__(CT) append_kernel(AppendArgs A) {
+  const int b = blockIdx.x, len = A.lens[b], at = len >> A.lp;
+  if (len < 0 || at >= A.width) return;
+  const int id = A.tables[(size_t)b * A.t_sb + at], slot = len & ((1 << A.lp) - 1);
+  if (id < 0 || id >= A.num_pages) return;
+  const int cpr = A.d / 8;
+  for (int t = threadIdx.x; t < A.hkv * cpr; t += CT) {
+    const int h = t / cpr, c = t % cpr;
+    const u32x4 kw = *(gu32x4*)(A.kr + (size_t)b * A.k_sb + (size_t)h * A.k_sh + 8 * c);
+    const u32x4 vw = *(gu32x4*)(A.vr + (size_t)b * A.v_sb + (size_t)h * A.v_sh + 8 * c);
+    const size_t head = (size_t)id * A.hkv + h, p = ((head << A.lp) + slot) * A.d + 8 * c;
+    if (A.bounds) {
+      uint16_t* bd = A.bounds + head * 2 * A.d + 8 * c;
+      u32x4 lo = kw, hi = kw;
+      if (slot > 0) {
+        float f[8], lf[8], hf[8];
+        to_f32x8<F16>(kw, f);
+        to_f32x8<F16>(*(gu32x4*)bd, lf);
+        to_f32x8<F16>(*(gu32x4*)(bd + A.d), hf);
+#pragma unroll
+        for (int i = 0; i < 8; i++) lf[i] = least(lf[i], f[i]), hf[i] = greatest(hf[i], f[i]);
+        lo = from_f32x8<F16>(lf);
+        hi = from_f32x8<F16>(hf);
+      }
+      *reinterpret_cast<u32x4*>(bd) = lo;
+      *reinterpret_cast<u32x4*>(bd + A.d) = hi;
+    }
+    *reinterpret_cast<u32x4*>(A.k + p) = kw;
+    *reinterpret_cast<u32x4*>(A.v + p) = vw;
+  }
+}
+
+// ------------------------------------------------------------------ attention over pages
+// One query token a sequence: o = softmax(scale q K^T) V over keys in pages, one pass with a running
+// maximum m, sum l and unnormalised output, in base 2 (scores times scale * log2 e). A workgroup takes
+// a chunk of keys for a tile of query rows of one kv head and leaves (m, l, o) of it; combine_kernel
+// joins the chunks. Rows that read the same keys share a tile: every query of every sequence for the
+// shared prefix, so its K and V are read once for 64 rows; the query heads of one kv head for a
+// sequence's own rows.
+//
+// The four waves of a workgroup take 32-key steps in turn and never wait for each other until the
+// chunk's end: each has two stages of LDS for its steps (K and V rows, moved by 1 KB DMA
+// instructions), so the next step's rows are in flight while this one's are multiplied. A row's
+// 16-byte pieces are XOR-swizzled with the row (applied where the DMA reads), so that the 16 rows of
+// a fragment read fall in distinct banks.
+//
+// Scores come transposed, S^T = K Q^T: a lane holds 4 keys of each 16-key tile for one query row, so
+// the softmax needs one reduction over the four lane groups, and its probabilities are already the
+// operand of O^T = V^T P^T, whose V^T comes from LDS by transpose reads in the same key order. The
+// probabilities are rounded to 16 bits for that product (a relative 2^-9 (bf16) of each term, as
+// much as the output's own rounding); maxima, sums and outputs stay in 32 bits.
+constexpr int AW = 4;     // waves
+constexpr int KS = 32;    // keys a step
+constexpr int STAGES = 2;
+
+#define PG_AWAIT(n) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(n) : "memory")
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+template <bool F16>
+__device__ __forceinline__ f32x4 mma(const u32x4& a, const u32x4& b, f32x4 c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return mfma_16x16x32(a, b, c);
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (F16)
+    return (uint32_t)__builtin_bit_cast(unsigned short, (_Float16)lo) |
+           (uint32_t)__builtin_bit_cast(unsigned short, (_Float16)hi) << 16;
+  else
+    return pack_bf2(lo, hi);
+}
+// maximum and sum over the four 16-lane groups (lanes l, l + 16, l + 32, l + 48), in every group
+__device__ __forceinline__ float groups_max(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float groups_sum(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// LDS bytes of one stage of one wave: KS rows of K, then KS rows of V
+template <int D>
+constexpr uint32_t stage_bytes = 2u * KS * D * 2;
+// the swizzle of a row's 16-byte pieces (D / 8 of them): 256-byte rows all start at the same bank,
+// 128-byte ones in pairs
+template <int D>
+__device__ __forceinline__ int swz(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
+
+// Keys [k_lo, k_hi) of `table` (page ids), kv head h, for RB * 16 query rows whose fragments are qf:
+// running maximum, sum (both for query row r16 of each block, the same in every lane group) and
+// output (lane: dims 16 dt + 4 kg + e of row r16). Returns whether a page id was outside the pool
+// (page 0 was read in its place).
+template <bool F16, int D, int RB>
+__device__ __forceinline__ bool attend(const AttnArgs& A, const int* table, int h, int k_lo, int k_hi, uint32_t lds,
+                                       int wv, int lane, const u32x4 (&qf)[RB][D / 32], float (&m)[RB], float (&l)[RB],
+                                       f32x4 (&o)[RB][D / 16]) {
+  typedef short v4s __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) v4s lds_v4s;
+  typedef const __attribute__((address_space(3))) u32x4 lds_u32x4;
+  constexpr int CPR = D / 8, RPI = 64 / CPR, NI = KS / RPI;  // pieces a row, rows a DMA instruction, instructions
+  constexpr uint32_t VOFF = KS * D * 2;
+  const int r16 = lane & 15, kg = lane >> 4, pmask = (1 << A.lp) - 1;
+  const size_t page_elems = ((size_t)A.hkv << A.lp) * D, head_elems = ((size_t)h << A.lp) * D;
+  bool bad = false;
+  // page ids of 64 pages at a time, one a lane
+  int win0 = k_lo >> A.lp;
+  const int last_page = (k_hi - 1) >> A.lp;
+  typedef const __attribute__((address_space(1))) int gint;
+  int win = *(gint*)(table + min(win0 + lane, last_page));
+  auto page_id = [&](int at) {
+    if (at - win0 >= 64) {
+      win0 = at;
+      win = *(gint*)(table + min(win0 + lane, last_page));
+    }
+    const int id = __builtin_amdgcn_readlane(win, at - win0);
+    if (id >= 0 && id < A.num_pages) return id;
+    bad = true;
+    return 0;
+  };
+  // the rows of the step at key k0 into stage s: K first, then V
+  auto fetch = [&](int k0, int s) {
+    const int at = k0 >> A.lp;
+    const size_t base0 = (size_t)page_id(at) * page_elems + head_elems;
+    // pages of 16 rows: the step's second half lies in the next page, if it has any key
+    const bool two = A.lp == 4 && k0 + 16 < k_hi;
+    const size_t base1 = two ? (size_t)page_id(at + 1) * page_elems + head_elems : base0;
+    const uint32_t dst = lds + s * stage_bytes<D>;
+#pragma unroll
+    for (int kv = 0; kv < 2; kv++) {
+      const uint16_t* pool = kv ? A.v : A.k;
+#pragma unroll
+      for (int i = 0; i < NI; i++) {
+        const int row = RPI * i + lane / CPR;
+        const int key = min(k0 + row, k_hi - 1);  // (rows past the end repeat the last key; their scores are masked)
+        const uint16_t* src = pool + (i * RPI < 16 ? base0 : base1) + (size_t)((key & pmask) * D + 8 * ((lane % CPR) ^ swz<D>(row)));
+        dma16(src, __builtin_amdgcn_readfirstlane(dst + kv * VOFF + 1024u * i));
+      }
+    }
+  };
+#pragma unroll
+  for (int rb = 0; rb < RB; rb++) {
+    m[rb] = -INFINITY;
+    l[rb] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < D / 16; dt++) o[rb][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  // fragment addresses in a stage: K row r16 (+ 16 t), pieces 4 ks + kg; V keys 4 kg + r16 / 4 (+ 16 t),
+  // dims 16 dt + 4 (r16 % 4) .. + 3
+  const uint32_t ka = r16 * (2 * D) + 16 * (kg ^ swz<D>(r16));
+  const int vrow = 4 * kg + (r16 >> 2);
+  const uint32_t va = VOFF + vrow * (2 * D) + 16 * (((r16 & 3) >> 1) ^ swz<D>(vrow)) + 8 * (r16 & 1);
+  const float c = A.scale_log2;
+  int k0 = k_lo + KS * wv, s = 0;
+  if (k0 < k_hi) fetch(k0, 0);
+  for (; k0 < k_hi; k0 += KS * AW, s ^= 1) {
+    const bool more = k0 + KS * AW < k_hi;
+    // the other stage's last reads are done before the DMA writes there
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (more) fetch(k0 + KS * AW, s ^ 1);
+    const uint32_t st = lds + s * stage_bytes<D>;
+    if (more) PG_AWAIT(3 * NI); else PG_AWAIT(NI);  // K is there
+    f32x4 sc[RB][2];
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+      u32x4 kf[D / 32];
+#pragma unroll
+      for (int ks = 0; ks < D / 32; ks++) kf[ks] = *(lds_u32x4*)(uintptr_t)(st + ((ka ^ (64u * ks)) + 16u * 2 * D * t));
+#pragma unroll
+      for (int rb = 0; rb < RB; rb++) {
+        f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < D / 32; ks++) a = mma<F16>(kf[ks], qf[rb][ks], a);
+#pragma unroll
+        for (int e = 0; e < 4; e++) a[e] *= c;
+        sc[rb][t] = a;
+      }
+    }
+    if (k0 + KS > k_hi) {
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (k0 + 16 * t + 4 * kg + e >= k_hi)
+#pragma unroll
+            for (int rb = 0; rb < RB; rb++) sc[rb][t][e] = -INFINITY;
+    }
+    u32x4 pf[RB];
+#pragma unroll
+    for (int rb = 0; rb < RB; rb++) {
+      float mx = fmaxf(fmaxf(fmaxf(sc[rb][0][0], sc[rb][0][1]), fmaxf(sc[rb][0][2], sc[rb][0][3])),
+                       fmaxf(fmaxf(sc[rb][1][0], sc[rb][1][1]), fmaxf(sc[rb][1][2], sc[rb][1][3])));
+      mx = fmaxf(m[rb], groups_max(mx));
+      if (__any(mx > m[rb])) {  // (wave-uniform: a step that raises no maximum rescales nothing)
+        const float al = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rb] - mx);
+        l[rb] *= al;
+#pragma unroll
+        for (int dt = 0; dt < D / 16; dt++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) o[rb][dt][e] *= al;
+        m[rb] = mx;
+      }
+      const float base = m[rb] == -INFINITY ? 0.f : m[rb];
+      float p[8], sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        p[i] = __builtin_amdgcn_exp2f(sc[rb][i >> 2][i & 3] - base);
+        sum += p[i];
+      }
+      l[rb] += sum;  // (of this lane group's keys; joined after the last step)
+#pragma unroll
+      for (int i = 0; i < 4; i++) pf[rb][i] = pack2<F16>(p[2 * i], p[2 * i + 1]);
+    }
+    if (more) PG_AWAIT(2 * NI); else PG_AWAIT(0);  // V is there
+#pragma unroll
+    for (int dt = 0; dt < D / 16; dt++) {
+      const uint32_t a = st + (va ^ (32u * dt));
+      const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(uintptr_t)a));
+      const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(uintptr_t)(a + 16u * 2 * D)));
+      const u32x4 vf = u32x4{lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+      for (int rb = 0; rb < RB; rb++) o[rb][dt] = mma<F16>(vf, pf[rb], o[rb][dt]);
+    }
+  }
+#pragma unroll
+  for (int rb = 0; rb < RB; rb++) l[rb] = groups_sum(l[rb]);
+  return bad;
+}
+
+// One chunk of keys for RB * 16 query rows from row0 of `rows` rows of kv head h (row r: query head
+// h G + r % G of sequence b0 + r / G), to partial `slot`.
+template <bool F16, int D, int RB>
+__device__ void chunk(const AttnArgs& A, const int* table, int h, int b0, int row0, int rows, int k_lo, int k_hi, int slot,
+                      uint32_t lds, float (*s_m)[64], float (*s_l)[64]) {
+  typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, kg = lane >> 4;
+  u32x4 qf[RB][D / 32];
+#pragma unroll
+  for (int rb = 0; rb < RB; rb++) {
+    const int r = min(row0 + 16 * rb + r16, rows - 1);  // (rows past the end repeat the last one and are not stored)
+    const uint16_t* q = A.q + (size_t)(b0 + r / A.g) * A.q_sb + (size_t)(h * A.g + r % A.g) * A.q_sh;
+#pragma unroll
+    for (int ks = 0; ks < D / 32; ks++) qf[rb][ks] = *(gu32x4*)(q + 32 * ks + 8 * kg);
+  }
+  float m[RB], l[RB];
+  f32x4 o[RB][D / 16];
+  constexpr uint32_t WAVE = STAGES * stage_bytes<D>;
+  static_assert(RB * 16 * D * 4 <= (int)WAVE, "a wave's output fits its stages");
+  const uint32_t mine = lds + WAVE * wv;
+  const bool bad = attend<F16, D, RB>(A, table, h, k_lo, k_hi, mine, wv, lane, qf, m, l, o);
+  // ---- join the waves: each scales its output to the rows' common maximum and leaves it in its stages
+  // (row: D / 4 pieces of 16 bytes, swizzled with the row), then all add the four up
+  if (kg == 0)
+#pragma unroll
+    for (int rb = 0; rb < RB; rb++) {
+      s_m[wv][16 * rb + r16] = m[rb];
+      s_l[wv][16 * rb + r16] = bad ? NAN : l[rb];
+    }
+  __syncthreads();
+#pragma unroll
+  for (int rb = 0; rb < RB; rb++) {
+    const int r = 16 * rb + r16;
+    float mx = s_m[0][r];
+#pragma unroll
+    for (int w = 1; w < AW; w++) mx = fmaxf(mx, s_m[w][r]);
+    const float f = m[rb] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rb] - mx);
+#pragma unroll
+    for (int dt = 0; dt < D / 16; dt++) {
+      f32x4 x = o[rb][dt];
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[e] *= f;
+      *(lds_f32x4*)(uintptr_t)(mine + r * (4 * D) + 16 * ((4 * dt + kg) ^ r16)) = x;
+    }
+  }
+  __syncthreads();
+  constexpr int PPR = D / 4;  // 16-byte pieces a row
+  for (int i = tid; i < RB * 16 * PPR; i += 64 * AW) {
+    const int r = i / PPR, p = i % PPR, row = row0 + r;
+    if (row >= rows) break;
+    f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < AW; w++) x += *(lds_f32x4*)(uintptr_t)(lds + WAVE * w + r * (4 * D) + 16 * (p ^ (r & 15)));
+    const size_t at = (size_t)slot * A.batch * A.hq + (size_t)(b0 + row / A.g) * A.hq + h * A.g + row % A.g;
+    *reinterpret_cast<f32x4*>(A.part_o + at * D + 4 * p) = x;
+    if (p == 0) {
+      float mx = s_m[0][r], sum = 0.f;
+#pragma unroll
+      for (int w = 1; w < AW; w++) mx = fmaxf(mx, s_m[w][r]);
+#pragma unroll
+      for (int w = 0; w < AW; w++) {
+        const float mw = s_m[w][r];
+        sum += s_l[w][r] * (mw == -INFINITY ? (s_l[w][r] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(mw - mx));
+      }
+      A.part_ml[at] = make_float2(mx, sum);
+    }
+  }
+}
+
+// keys of one part of `parts` of `len` keys, in whole steps of the workgroup's four waves
+__device__ __forceinline__ int part_keys(int len, int parts) {
+  constexpr int U = KS * AW;
+  return ((len + parts - 1) / parts + U - 1) / U * U;
+}
+
+template <bool F16, int D, int RB>
+__global__ void __launch_bounds__(64 * AW) attn_kernel(AttnArgs A) {
+  __shared__ __align__(1024) uint8_t s_kv[AW * STAGES * stage_bytes<D>];
+  __shared__ float s_m[AW][64], s_l[AW][64];
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&s_kv[0];
+  int id = blockIdx.x;
+  const int h = id % A.hkv;  // (fastest: with 8 kv heads each XCD reads one head's rows)
+  id /= A.hkv;
+  if (id < A.prefix_tiles * A.np) {
+    const int tile = id % A.prefix_tiles, part = id / A.prefix_tiles;
+    const int ch = part_keys(A.prefix_len, A.np), lo = part * ch, hi = min(A.prefix_len, lo + ch);
+    if (lo >= hi) {
+      // (the last parts of a prefix that does not fill them all)
+      for (int r = threadIdx.x; r < 16 * RB; r += 64 * AW) {
+        const int row = 16 * RB * tile + r;
+        if (row < A.batch * A.g)
+          A.part_ml[(size_t)part * A.batch * A.hq + (size_t)(row / A.g) * A.hq + h * A.g + row % A.g] = make_float2(-INFINITY, 0.f);
+      }
+      return;
+    }
+    chunk<F16, D, RB>(A, A.prefix_pages, h, 0, 16 * RB * tile, A.batch * A.g, lo, hi, part, lds, s_m, s_l);
+    return;
+  }
+  id -= A.prefix_tiles * A.np;
+  const int tile = id % A.own_tiles;
+  id /= A.own_tiles;
+  const int b = id % A.batch, part = id / A.batch;
+  const int len = max(0, min(A.lens[b] + A.len_add, A.width << A.lp));
+  const int ch = part_keys(len, A.ns), lo = part * ch, hi = min(len, lo + ch);
+  if (lo >= hi) {
+    const int r = 16 * tile + threadIdx.x;
+    if (threadIdx.x < 16 && r < A.g)
+      A.part_ml[(size_t)(A.np + part) * A.batch * A.hq + (size_t)b * A.hq + h * A.g + r] = make_float2(-INFINITY, 0.f);
+    return;
+  }
+  chunk<F16, D, 1>(A, A.tables + (size_t)b * A.t_sb + (size_t)h * A.t_sh, h, b, 16 * tile, A.g, lo, hi, A.np + part, lds, s_m,
+                   s_l);
+}
+
+// Workgroup (query head, sequence): the parts' outputs, scaled to their common maximum, over their
+// sums. Rows without a key give zeros. Eight (D = 128) or sixteen groups of lanes take the parts in
+// turn; the groups are added in order, so a result does not depend on timing.
+template <bool F16, int D>
+__global__ void __launch_bounds__(256) combine_kernel(AttnArgs A) {
+  constexpr int LPR = D / 4, GROUPS = 256 / LPR;
+  __shared__ f32x4 s_o[GROUPS][LPR];
+  __shared__ float s_l[GROUPS];
+  const int hq = blockIdx.x, b = blockIdx.y, parts = A.np + A.ns, lane = threadIdx.x % LPR, grp = threadIdx.x / LPR;
+  const size_t row = (size_t)b * A.hq + hq, step = (size_t)A.batch * A.hq;
+  float mx = -INFINITY;
+  for (int p = 0; p < parts; p++) mx = fmaxf(mx, A.part_ml[row + step * p].x);
+  const float base = mx == -INFINITY ? 0.f : mx;
+  f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
+  float l = 0.f;
+  for (int p = grp; p < parts; p += GROUPS) {
+    const float2 ml = A.part_ml[row + step * p];
+    if (ml.y == 0.f) continue;  // (no key: its output was not written)
+    const float w = __builtin_amdgcn_exp2f(ml.x - base);
+    const f32x4 y = *reinterpret_cast<const f32x4*>(A.part_o + (row + step * p) * D + 4 * lane);
+    l += w * ml.y;
+#pragma unroll
+    for (int e = 0; e < 4; e++) x[e] += w * y[e];
+  }
+  s_o[grp][lane] = x;
+  if (lane == 0) s_l[grp] = l;
+  __syncthreads();
+  if (grp > 0) return;
+  for (int g = 1; g < GROUPS; g++) {
+    x += s_o[g][lane];
+    l += s_l[g];
+  }
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  u32x2 w;
+  w.x = pack2<F16>(x[0] * inv, x[1] * inv);
+  w.y = pack2<F16>(x[2] * inv, x[3] * inv);
+  *reinterpret_cast<u32x2*>(A.out + (size_t)b * A.o_sb + (size_t)hq * A.o_sh + 4 * lane) = w;
+}
+
+// ------------------------------------------------------------------ choosing pages
+// The score of a page for the queries of one kv head is the most that their products with any of its
+// keys can add up to, given the bounds lo <= key <= hi of each dim:
+//   sum over queries and dims of max(q lo, q hi) = sum over dims of hi sum(max(q, 0)) + lo sum(min(q, 0)),
+// two products a dim whatever the number of queries. It is summed in 64 bits, where these 16-bit
+// values' products and sums are exact but for far smaller terms, so that the choice does not hang on
+// the order of the additions. Chosen are the last page and the top - 1 best others, the lower
+// of equals first; a score that is not a number counts as the greatest.
+//
+// One workgroup a (kv head, sequence): 16 lanes take a page (8 dims each at 128), the scores go to LDS
+// as unsigned 64-bit keys in the order of the scores, a radix selection by 8 bits finds the last key
+// that is chosen, and a scan writes the chosen pages in ascending order.
+constexpr int ST = 1024;              // threads
+
+__device__ __forceinline__ uint64_t order_key(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x + 0.0);  // (-0 counts as 0)
+  if (x != x) return ~0ull;
+  return u >> 63 ? ~u : u | 1ull << 63;
+}
+
+template <bool F16, int D>
+__global__ void __launch_bounds__(ST) select_kernel(SelectArgs A) {
+  constexpr int LPP = D / 8, PPW = ST / LPP;  // lanes a page, pages at a time
+  extern __shared__ __align__(16) uint64_t s_key[];  // [width]
+  __shared__ double s_q[2][D];
+  __shared__ uint32_t s_hist[256];
+  __shared__ uint32_t s_sel[2];    // the digit chosen, keys still wanted in it
+  __shared__ uint32_t s_cnt[2][ST / 64];
+  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  const int len = max(0, min(A.lens[b] + A.len_add, A.width << A.lp)), used = (len + (1 << A.lp) - 1) >> A.lp;
+  const int* table = A.tables + (size_t)b * A.t_sb;
+  int* chosen = A.chosen + ((size_t)b * A.hkv + h) * A.top;
+  int* pages = A.pages + ((size_t)b * A.hkv + h) * A.top;
+  const int count = min(used, A.top);
+  if (h == 0 && tid == 0) A.sub_lens[b] = count == 0 ? 0 : ((count - 1) << A.lp) + ((len - 1) & ((1 << A.lp) - 1)) + 1;
+  for (int i = count + tid; i < A.top; i += ST) chosen[i] = -1, pages[i] = -1;
+  if (used <= A.top) {
+    for (int i = tid; i < used; i += ST) chosen[i] = i, pages[i] = table[i];
+    return;
+  }
+  if (tid < D) {
+    double pos = 0.0, neg = 0.0;
+    for (int g = 0; g < A.g; g++) {
+      const float x = to_f32<F16>(*(gu16*)(A.q + (size_t)b * A.q_sb + (size_t)(h * A.g + g) * A.q_sh + tid));
+      if (x > 0.f) pos += x; else neg += x;  // (not a number: in neg, and so in every score)
+    }
+    s_q[0][tid] = neg;
+    s_q[1][tid] = pos;
+  }
+  __syncthreads();
+  {
+    const int c = tid % LPP;
+    double ql[8], qh[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) ql[i] = s_q[0][8 * c + i], qh[i] = s_q[1][8 * c + i];
+    for (int p = tid / LPP; p < used - 1; p += PPW) {
+      const int id = table[p];
+      double x = INFINITY;  // a page outside the pool is chosen: its sequence's outputs are then not numbers
+      if (id >= 0 && id < A.num_pages) {
+        const uint16_t* bd = A.bounds + ((size_t)id * A.hkv + h) * 2 * D + 8 * c;
+        float lo[8], hi[8];
+        to_f32x8<F16>(*(gu32x4*)bd, lo);
+        to_f32x8<F16>(*(gu32x4*)(bd + D), hi);
+        x = 0.0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          x = fma((double)lo[i], ql[i], x);
+          x = fma((double)hi[i], qh[i], x);
+        }
+      }
+#pragma unroll
+      for (int off = LPP / 2; off > 0; off >>= 1) x += __shfl_xor(x, off, LPP);
+      if (c == 0) s_key[p] = order_key(x);
+    }
+  }
+  // ---- the want-th greatest of used - 1 keys, 8 bits at a time from the top
+  const int n = used - 1;
+  uint32_t want = A.top - 1;
+  uint64_t prefix = 0, mask = 0;
+  if (want > 0)
+    for (int shift = 56; shift >= 0; shift -= 8) {
+      if (tid < 256) s_hist[tid] = 0;
+      __syncthreads();
+      for (int i = tid; i < n; i += ST) {
+        const uint64_t k = s_key[i];
+        if ((k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & 255], 1u);
+      }
+      __syncthreads();
+      if (wv == 0) {
+        // lane: digits 255 - 4 lane .. 252 - 4 lane, from the greatest down
+        uint32_t c4[4], sum = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) sum += c4[i] = s_hist[255 - 4 * lane - i];
+        uint32_t before = sum;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+          const uint32_t y = __shfl_up(before, off, 64);
+          if (lane >= off) before += y;
+        }
+        before -= sum;  // keys with a greater digit than this lane's
+        if (before < want && before + sum >= want) {
+          uint32_t at = before;
+          int i = 0;
+          while (at + c4[i] < want) at += c4[i++];
+          s_sel[0] = 255 - 4 * lane - i;
+          s_sel[1] = want - at;
+        }
+      }
+      __syncthreads();
+      prefix |= (uint64_t)s_sel[0] << shift;
+      mask |= 255ull << shift;
+      want = s_sel[1];
+    }
+  else
+    __syncthreads();
+  // ---- keys above the last chosen one, and the first `want` of its equals, in ascending order
+  uint32_t eq0 = 0, out0 = 0;
+  for (int i0 = 0; i0 < n && A.top > 1; i0 += ST) {
+    const int i = i0 + tid;
+    const uint64_t k = i < n ? s_key[i] : 0;
+    const bool gt = i < n && k > prefix, eq = i < n && k == prefix;
+    const uint64_t below = (1ull << lane) - 1;
+    const uint64_t be = __ballot(eq), bg = __ballot(gt);
+    if (lane == 0) s_cnt[0][wv] = __popcll(be), s_cnt[1][wv] = __popcll(bg);
+    __syncthreads();
+    uint32_t e = eq0, g = 0, all_e = 0, all_g = 0;
+    for (int w = 0; w < ST / 64; w++) {
+      if (w < wv) e += s_cnt[0][w], g += s_cnt[1][w];
+      all_e += s_cnt[0][w];
+      all_g += s_cnt[1][w];
+    }
+    e += __popcll(be & below);
+    g += __popcll(bg & below);
+    // of the equals before this one, at most `want` were chosen
+    if (gt || (eq && e < want)) {
+      const uint32_t at = out0 + g + (min(e, want) - min(eq0, want));
+      chosen[at] = i;
+      pages[at] = table[i];
+    }
+    out0 += all_g + min(eq0 + all_e, want) - min(eq0, want);
+    eq0 += all_e;
+    __syncthreads();
+  }
+  if (tid == 0) chosen[A.top - 1] = n, pages[A.top - 1] = table[n];
+}
+
+// ------------------------------------------------------------------ launches
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+static bool pool_ok(const MqPagePool* p, bool need_bounds) {
+  if (!p || !p->k || !p->v || (need_bounds && !p->bounds)) return false;
+  if (!aligned16(p->k) || !aligned16(p->v) || !aligned16(p->bounds)) return false;
+  if (p->num_layers < 1 || p->num_layers > 65535 || p->num_pages < 1 || p->num_kv_heads < 1 || p->num_kv_heads > 1024)
+    return false;
+  if (p->page_size < 16 || p->page_size > 256 || (p->page_size & (p->page_size - 1))) return false;
+  return (p->head_dim == 64 || p->head_dim == 128) && (p->dtype == MQ_BF16 || p->dtype == MQ_FP16);
+}
+static bool ids_ok(const int* ids, int n, int num_pages) {
+  for (int i = 0; i < n; i++)
+    if (ids[i] < 0 || ids[i] >= num_pages) return false;
+  return true;
+}
+static int log2_of(int x) { return __builtin_ctz((unsigned)x); }
+
+template <int N>
+static void copy_launch(const MqPagePool& P, const int* src, const int* dst, int n, hipStream_t stream) {
+  CopyArgs<N> A;
+  A.base[0] = P.k; A.base[1] = P.v; A.base[2] = P.bounds;
+  A.page_bytes = (uint32_t)P.num_kv_heads * P.page_size * P.head_dim * 2;
+  A.bounds_bytes = (uint32_t)P.num_kv_heads * 2 * P.head_dim * 2;
+  A.per_page = (A.page_bytes + CB - 1) / CB;
+  A.num_pages = P.num_pages; A.n = n;
+  for (int i = 0; i < n; i++) A.ids[i] = make_int2(src[i], dst[i]);
+  const uint32_t parts = 2 * A.per_page + (P.bounds ? (A.bounds_bytes + CB - 1) / CB : 0);
+  copy_kernel<N><<<dim3(parts, n, P.num_layers), CT, 0, stream>>>(A);
+}
+
+template <int N, bool IN>
+static void move_launch(const MqPagePool& P, const int* pages, int n, int first, int length, const void* kc, const void* vc,
+                        int max_seq, hipStream_t stream) {
+  MoveArgs<N> A;
+  A.k = static_cast<uint16_t*>(P.k); A.v = static_cast<uint16_t*>(P.v); A.bounds = static_cast<uint16_t*>(P.bounds);
+  A.kc = static_cast<uint16_t*>(const_cast<void*>(kc)); A.vc = static_cast<uint16_t*>(const_cast<void*>(vc));
+  A.num_pages = P.num_pages; A.hkv = P.num_kv_heads; A.page = P.page_size; A.d = P.head_dim;
+  A.max_seq = max_seq; A.first = first; A.length = length;
+  memcpy(A.ids, pages, sizeof(int) * n);
+  const dim3 grid(P.num_kv_heads, n, P.num_layers);
+  if (P.dtype == MQ_FP16)
+    move_kernel<N, IN, true><<<grid, CT, 0, stream>>>(A);
+  else
+    move_kernel<N, IN, false><<<grid, CT, 0, stream>>>(A);
+}
+
+// Both directions between a contiguous cache and pages, LIST_LONG pages a launch.
+template <bool IN>
+static int move(const MqPagePool* P, const int* pages, int length, const void* kc, const void* vc, int max_seq,
+                hipStream_t stream) {
+  if (!pool_ok(P, false) || !pages || !kc || !vc || !aligned16(kc) || !aligned16(vc) || length < 1 || max_seq < length)
+    return MQ_ERR_ARG;
+  const int n = (length + P->page_size - 1) / P->page_size;
+  if (!ids_ok(pages, n, P->num_pages)) return MQ_ERR_ARG;
+  (void)hipGetLastError();  // clear an error left by an unrelated earlier call
+  for (int i = 0; i < n; i += LIST_LONG) {
+    const int m = n - i < LIST_LONG ? n - i : LIST_LONG, first = i * P->page_size;
+    if (m <= LIST_SHORT)
+      move_launch<LIST_SHORT, IN>(*P, pages + i, m, first, length, kc, vc, max_seq, stream);
+    else
+      move_launch<LIST_LONG, IN>(*P, pages + i, m, first, length, kc, vc, max_seq, stream);
+    if (hipGetLastError() != hipSuccess) return MQ_ERR_HIP;
+  }
+  return MQ_OK;
+}
+
+int append_rows(const AppendArgs& A, bool f16, hipStream_t stream) {
+  if (f16)
+    append_kernel<true><<<A.batch, CT, 0, stream>>>(A);
+  else
+    append_kernel<false><<<A.batch, CT, 0, stream>>>(A);
+  return hipGetLastError() == hipSuccess ? MQ_OK : MQ_ERR_HIP;
+}
+
+// How an attention call is split. Query rows of the prefix go in tiles of 16, 32 or 64, so that its
+// keys are read as few times as there are tiles; a sequence's own rows are shared by its G query
+// heads a kv head only, in tiles of 16. Keys are split until the launch has about two workgroups a
+// CU (one is resident, the next follows), in parts of at least 128 keys (a step for each wave).
+AttnPlan plan_attention(int batch, int hkv, int g, int d, int prefix_len, int max_len) {
+  AttnPlan p{};
+  constexpr int UNIT = KS * AW, WANT = 512, MAX_PARTS = 64;
+  const int rows = batch * g;
+  p.rb = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  p.own_tiles = (g + 15) / 16;
+  auto parts = [&](int len, long long tiles) {
+    const int most = (len + UNIT - 1) / UNIT;
+    long long n = (WANT + tiles - 1) / tiles;
+    if (n > most) n = most;
+    return (int)(n > MAX_PARTS ? MAX_PARTS : n);
+  };
+  if (prefix_len > 0) {
+    p.prefix_tiles = (rows + 16 * p.rb - 1) / (16 * p.rb);
+    p.np = parts(prefix_len, (long long)hkv * p.prefix_tiles);
+  }
+  if (max_len > 0) p.ns = parts(max_len, (long long)batch * hkv * p.own_tiles);
+  const size_t rows_all = (size_t)(p.np + p.ns) * batch * hkv * g;
+  p.out_bytes = (rows_all * d * 4 + 255) / 256 * 256;
+  p.bytes = p.out_bytes + (rows_all * 8 + 255) / 256 * 256;
+  return p;
+}
+
+template <bool F16, int D>
+static void attn_launch(const AttnArgs& A, int rb, unsigned blocks, hipStream_t stream) {
+  if (blocks > 0) {
+    switch (rb) {
+      case 1: attn_kernel<F16, D, 1><<<blocks, 64 * AW, 0, stream>>>(A); break;
+      case 2: attn_kernel<F16, D, 2><<<blocks, 64 * AW, 0, stream>>>(A); break;
+      default: attn_kernel<F16, D, 4><<<blocks, 64 * AW, 0, stream>>>(A); break;
+    }
+  }
+  combine_kernel<F16, D><<<dim3(A.hq, A.batch), 256, 0, stream>>>(A);
+}
+
+// Both launches of an attention; A without its split and partial results, which come from `p` and
+// `ws` (plan_attention's bytes).
+int run_attention(AttnArgs A, const AttnPlan& p, int d, bool f16, void* ws, hipStream_t stream) {
+  A.prefix_tiles = p.prefix_tiles; A.np = p.np; A.own_tiles = p.own_tiles; A.ns = p.ns;
+  A.part_o = static_cast<float*>(ws);
+  A.part_ml = reinterpret_cast<float2*>(static_cast<char*>(ws) + p.out_bytes);
+  const long long blocks = (long long)A.hkv * ((long long)p.prefix_tiles * p.np + (long long)p.own_tiles * A.batch * p.ns);
+  if (blocks > 0x7fffffff) return MQ_ERR_ARG;
+  if (d == 128)
+    f16 ? attn_launch<true, 128>(A, p.rb, (unsigned)blocks, stream) : attn_launch<false, 128>(A, p.rb, (unsigned)blocks, stream);
+  else
+    f16 ? attn_launch<true, 64>(A, p.rb, (unsigned)blocks, stream) : attn_launch<false, 64>(A, p.rb, (unsigned)blocks, stream);
+  return hipGetLastError() == hipSuccess ? MQ_OK : MQ_ERR_HIP;
+}
+
+static bool rows_ok(const void* p, int64_t sb, int64_t sh) { return p && aligned16(p) && sb % 8 == 0 && sh % 8 == 0; }
+
+// What both attentions ask of their common arguments.
+static bool attn_ok(const MqPagePool* P, bool sparse, const void* q, int64_t q_sb, int64_t q_sh, const void* out, int64_t o_sb,
+                    int64_t o_sh, int num_q_heads, int batch, const int* tables, int64_t t_sb, int width, const int* lens,
+                    float scale, const void* ws) {
+  return pool_ok(P, sparse) && rows_ok(q, q_sb, q_sh) && rows_ok(out, o_sb, o_sh) && batch >= 1 && batch <= 65535 &&
+         num_q_heads >= P->num_kv_heads && num_q_heads <= 65535 && num_q_heads % P->num_kv_heads == 0 && tables && lens &&
+         width >= 1 && width <= MQ_MAX_TABLE_WIDTH && t_sb >= 0 && scale > 0.f && isfinite(scale) && ws && aligned16(ws);
+}
+
+static AttnArgs attn_args(const MqPagePool& P, const void* q, int64_t q_sb, int64_t q_sh, void* out, int64_t o_sb,
+                          int64_t o_sh, int num_q_heads, int batch, float scale) {
+  AttnArgs A{};
+  A.k = static_cast<const uint16_t*>(P.k); A.v = static_cast<const uint16_t*>(P.v);
+  A.q = static_cast<const uint16_t*>(q); A.out = static_cast<uint16_t*>(out);
+  A.q_sb = q_sb; A.q_sh = q_sh; A.o_sb = o_sb; A.o_sh = o_sh;
+  A.num_pages = P.num_pages; A.hkv = P.num_kv_heads; A.hq = num_q_heads; A.g = num_q_heads / P.num_kv_heads;
+  A.lp = log2_of(P.page_size); A.batch = batch;
+  A.scale_log2 = scale * 1.44269504088896341f;
+  return A;
+}
+
+int shared_attention(const MqPagePool* P, const void* q, int64_t q_sb, int64_t q_sh, void* out, int64_t o_sb, int64_t o_sh,
+                     int num_q_heads, int batch, const int* prefix_pages, int prefix_len, const int* tables, int64_t t_sb,
+                     int width, const int* lens, int len_add, int max_len, float scale, void* ws, size_t ws_bytes,
+                     hipStream_t stream) {
+  if (!attn_ok(P, false, q, q_sb, q_sh, out, o_sb, o_sh, num_q_heads, batch, tables, t_sb, width, lens, scale, ws) ||
+      prefix_len < 0 || (prefix_len > 0 && !prefix_pages) || max_len < 0)
+    return MQ_ERR_ARG;
+  const AttnPlan p = plan_attention(batch, P->num_kv_heads, num_q_heads / P->num_kv_heads, P->head_dim, prefix_len, max_len);
+  if (ws_bytes < p.bytes) return MQ_ERR_ARG;
+  AttnArgs A = attn_args(*P, q, q_sb, q_sh, out, o_sb, o_sh, num_q_heads, batch, scale);
+  A.prefix_pages = prefix_pages; A.prefix_len = prefix_len;
+  A.tables = tables; A.t_sb = t_sb; A.width = width; A.lens = lens; A.len_add = len_add;
+  return run_attention(A, p, P->head_dim, P->dtype == MQ_FP16, ws, stream);
+}
+
+// The chosen pages and the rows in them, ahead of the attention's partial results in the workspace.
+static size_t chosen_bytes(int batch, int hkv, int top) { return ((size_t)batch * (hkv * (size_t)top + 1) * 4 + 255) / 256 * 256; }
+
+int sparse_attention(const MqPagePool* P, const void* q, int64_t q_sb, int64_t q_sh, void* out, int64_t o_sb, int64_t o_sh,
+                     int* chosen, int num_q_heads, int batch, const int* tables, int64_t t_sb, int width, const int* lens,
+                     int len_add, int top, float scale, void* ws, size_t ws_bytes, hipStream_t stream) {
+  if (!attn_ok(P, true, q, q_sb, q_sh, out, o_sb, o_sh, num_q_heads, batch, tables, t_sb, width, lens, scale, ws) || !chosen ||
+      top < 1 || top > MQ_MAX_TABLE_WIDTH)
+    return MQ_ERR_ARG;
+  const int most = top < width ? top : width, hkv = P->num_kv_heads, g = num_q_heads / hkv;
+  const AttnPlan p = plan_attention(batch, hkv, g, P->head_dim, 0, most * P->page_size);
+  const size_t head = chosen_bytes(batch, hkv, top);
+  if (ws_bytes < head + p.bytes) return MQ_ERR_ARG;
+  AttnArgs A = attn_args(*P, q, q_sb, q_sh, out, o_sb, o_sh, num_q_heads, batch, scale);
+  SelectArgs S{};
+  S.q = A.q; S.bounds = static_cast<const uint16_t*>(P->bounds);
+  S.q_sb = q_sb; S.q_sh = q_sh; S.t_sb = t_sb; S.tables = tables; S.lens = lens;
+  S.chosen = chosen; S.pages = static_cast<int*>(ws); S.sub_lens = S.pages + (size_t)batch * hkv * top;
+  S.num_pages = P->num_pages; S.hkv = hkv; S.g = g; S.lp = A.lp; S.width = width; S.top = top; S.len_add = len_add;
+  const dim3 grid(hkv, batch);
+  const size_t keys = (size_t)width * 8;
+  const bool f16 = P->dtype == MQ_FP16;
+  if (P->head_dim == 128)
+    f16 ? select_kernel<true, 128><<<grid, ST, keys, stream>>>(S) : select_kernel<false, 128><<<grid, ST, keys, stream>>>(S);
+  else
+    f16 ? select_kernel<true, 64><<<grid, ST, keys, stream>>>(S) : select_kernel<false, 64><<<grid, ST, keys, stream>>>(S);
+  if (hipGetLastError() != hipSuccess) return MQ_ERR_HIP;
+  A.tables = S.pages; A.t_sb = (int64_t)hkv * top; A.t_sh = top; A.width = top; A.lens = S.sub_lens;
+  return run_attention(A, p, P->head_dim, f16, static_cast<char*>(ws) + head, stream);
+}
+
+}  // namespace pg
+}  // namespace mq
+
+using namespace mq;
+using namespace mq::pg;
+
+extern "C" int mq_pages_copy(const MqPagePool* pool, const int* src, const int* dst, int n, hipStream_t stream) {
+  if (!pool_ok(pool, false) || n < 0 || (n > 0 && (!src || !dst))) return MQ_ERR_ARG;
+  if (!ids_ok(src, n, pool->num_pages) || !ids_ok(dst, n, pool->num_pages)) return MQ_ERR_ARG;
+  (void)hipGetLastError();  // clear an error left by an unrelated earlier call
+  for (int i = 0; i < n; i += LIST_LONG) {
+    const int m = n - i < LIST_LONG ? n - i : LIST_LONG;
+    if (m <= LIST_SHORT)
+      copy_launch<LIST_SHORT>(*pool, src + i, dst + i, m, stream);
+    else
+      copy_launch<LIST_LONG>(*pool, src + i, dst + i, m, stream);
+    if (hipGetLastError() != hipSuccess) return MQ_ERR_HIP;
+  }
+  return MQ_OK;
+}
+
+extern "C" int mq_pages_load(const MqPagePool* pool, const int* pages, int length, const void* k_cache, const void* v_cache,
+                             int max_seq_len, hipStream_t stream) {
+  return mq::pg::move<true>(pool, pages, length, k_cache, v_cache, max_seq_len, stream);
+}
+
+extern "C" int mq_pages_store(const MqPagePool* pool, const int* pages, int length, void* k_cache, void* v_cache,
+                              int max_seq_len, hipStream_t stream) {
+  return mq::pg::move<false>(pool, pages, length, k_cache, v_cache, max_seq_len, stream);
+}
+
+extern "C" int mq_pages_append(const MqPagePool* pool, const void* k, const void* v, long long k_sb, long long k_sh,
+                               long long v_sb, long long v_sh, const int* tables, long long table_stride, int width,
+                               const int* lens, int batch, hipStream_t stream) {
+  if (!pool_ok(pool, false) || pool->num_layers != 1 || !rows_ok(k, k_sb, k_sh) || !rows_ok(v, v_sb, v_sh) || !tables ||
+      table_stride < 0 || width < 1 || width > MQ_MAX_TABLE_WIDTH || !lens || batch < 1 || batch > 65535)
+    return MQ_ERR_ARG;
+  AppendArgs A{};
+  A.k = static_cast<uint16_t*>(pool->k); A.v = static_cast<uint16_t*>(pool->v); A.bounds = static_cast<uint16_t*>(pool->bounds);
+  A.kr = static_cast<const uint16_t*>(k); A.vr = static_cast<const uint16_t*>(v);
+  A.k_sb = k_sb; A.k_sh = k_sh; A.v_sb = v_sb; A.v_sh = v_sh; A.tables = tables; A.lens = lens; A.t_sb = table_stride;
+  A.num_pages = pool->num_pages; A.hkv = pool->num_kv_heads; A.lp = log2_of(pool->page_size); A.d = pool->head_dim;
+  A.width = width; A.batch = batch;
+  (void)hipGetLastError();  // clear an error left by an unrelated earlier call
+  return append_rows(A, pool->dtype == MQ_FP16, stream);
+}
+
+extern "C" int mq_attention_workspace(const MqPagePool* pool, int num_q_heads, int batch, int prefix_len, int max_len, int top,
+                                      size_t* bytes) {
+  if (!pool || !bytes || pool->num_kv_heads < 1 || num_q_heads < pool->num_kv_heads || num_q_heads % pool->num_kv_heads ||
+      batch < 1 || prefix_len < 0 || max_len < 0 || top < 0)
+    return MQ_ERR_ARG;
+  *bytes = plan_attention(batch, pool->num_kv_heads, num_q_heads / pool->num_kv_heads, pool->head_dim, prefix_len, max_len).bytes +
+           (top > 0 ? chosen_bytes(batch, pool->num_kv_heads, top) : 0);
+  return MQ_OK;
+}
+
+extern "C" int mq_shared_prefix_attention(const MqPagePool* pool, const void* q, long long q_sb, long long q_sh, void* out,
+                                          long long o_sb, long long o_sh, int num_q_heads, int batch, const int* prefix_pages,
+                                          int prefix_len, const int* tables, long long table_stride, int width,
+                                          const int* lens, int max_len, float scale, void* workspace,
+                                          size_t workspace_bytes, hipStream_t stream) {
+  (void)hipGetLastError();  // clear an error left by an unrelated earlier call
+  return shared_attention(pool, q, q_sb, q_sh, out, o_sb, o_sh, num_q_heads, batch, prefix_pages, prefix_len, tables,
+                          table_stride, width, lens, 0, max_len, scale, workspace, workspace_bytes, stream);
+}
+
+extern "C" int mq_sparse_attention(const MqPagePool* pool, const void* q, long long q_sb, long long q_sh, void* out,
+                                   long long o_sb, long long o_sh, int* chosen, int num_q_heads, int batch,
+                                   const int* tables, long long table_stride, int width, const int* lens, int top,
+                                   float scale, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  (void)hipGetLastError();  // clear an error left by an unrelated earlier call
+  return sparse_attention(pool, q, q_sb, q_sh, out, o_sb, o_sh, chosen, num_q_heads, batch, tables, table_stride, width, lens, 0,
+                          top, scale, workspace, workspace_bytes, stream);
+}
