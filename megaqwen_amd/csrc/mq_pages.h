@@ -43,10 +43,10 @@ struct SelectArgs {
   int num_pages, hkv, g, lp, width, top, len_add;
 };
 
-// How an attention call is split: query-row blocks of 16 a workgroup and row tiles, parts of the
+// How an attention call is split: the form and number of the prefix's row tiles, parts of the
 // prefix and of the own rows, and the workspace: the partial outputs, then the maxima and sums.
 struct AttnPlan {
-  int rb, prefix_tiles, np, own_tiles, ns;
+  int form, prefix_tiles, np, own_tiles, ns;
   size_t out_bytes, bytes;
 };
 AttnPlan plan_attention(int batch, int hkv, int g, int d, int prefix_len, int max_len);

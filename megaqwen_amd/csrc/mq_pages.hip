@@ -176,27 +176,31 @@ __global__ void __launch_bounds__(CT) append_kernel(AppendArgs A) {
 // ------------------------------------------------------------------ attention over pages
 // One query token a sequence: o = softmax(scale q K^T) V over keys in pages, one pass with a running
 // maximum m, sum l and unnormalised output, in base 2 (scores times scale * log2 e). A workgroup takes
-// a chunk of keys for a tile of query rows of one kv head and leaves (m, l, o) of it; combine_kernel
-// joins the chunks. Rows that read the same keys share a tile: every query of every sequence for the
-// shared prefix, so its K and V are read once for 64 rows; the query heads of one kv head for a
+// a part of the keys for a tile of query rows of one kv head and leaves (m, l, o) of it; combine_kernel
+// joins the parts. Rows that read the same keys share a tile: the queries of all sequences for the
+// shared prefix, so its K and V are read once for 128 rows, the query heads of one kv head for a
 // sequence's own rows.
 //
-// The four waves of a workgroup take 32-key steps in turn and never wait for each other until the
-// chunk's end: each has two stages of LDS for its steps (K and V rows, moved by 1 KB DMA
-// instructions), so the next step's rows are in flight while this one's are multiplied. A row's
-// 16-byte pieces are XOR-swizzled with the row (applied where the DMA reads), so that the 16 rows of
-// a fragment read fall in distinct banks.
+// K and V rows go to LDS by 1 KB DMA instructions; a row's 16-byte pieces are XOR-swizzled with the row
+// (applied where the DMA reads), so that the 16 rows of a fragment read fall in distinct banks. Every
+// form takes 64 KB of LDS and at most 256 registers (D = 128), so that two workgroups are resident on a
+// CU: while one starts, waits or joins its waves, the other streams, and parts of the prefix, which
+// are bound by the matrix units, run beside own rows, which are bound by memory.
 //
 // Scores come transposed, S^T = K Q^T: a lane holds 4 keys of each 16-key tile for one query row, so
 // the softmax needs one reduction over the four lane groups, and its probabilities are already the
 // operand of O^T = V^T P^T, whose V^T comes from LDS by transpose reads in the same key order. The
 // probabilities are rounded to 16 bits for that product (a relative 2^-9 (bf16) of each term, as
 // much as the output's own rounding); maxima, sums and outputs stay in 32 bits.
-constexpr int AW = 4;     // waves
-constexpr int KS = 32;    // keys a step
-constexpr int STAGES = 2;
+constexpr int AW = 4;   // waves
+constexpr int KS = 32;  // keys a wave takes at a time, of own rows
+constexpr int TS = 64;  // keys a workgroup takes at a time, of a prefix whose rows its waves share out
 
 #define PG_AWAIT(n) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(n) : "memory")
+// this wave's LDS reads are done
+#define PG_READ() asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory")
+// this wave's DMAs have landed and its LDS reads are done, for every wave of the workgroup
+#define PG_BARRIER() asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory")
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 template <bool F16>
@@ -228,162 +232,142 @@ __device__ __forceinline__ float groups_sum(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// LDS bytes of one stage of one wave: KS rows of K, then KS rows of V
-template <int D>
-constexpr uint32_t stage_bytes = 2u * KS * D * 2;
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4s lds_v4s;
+typedef const __attribute__((address_space(3))) u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
+typedef const __attribute__((address_space(1))) int gint;
+
 // the swizzle of a row's 16-byte pieces (D / 8 of them): 256-byte rows all start at the same bank,
 // 128-byte ones in pairs
 template <int D>
 __device__ __forceinline__ int swz(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
 
-// Keys [k_lo, k_hi) of `table` (page ids), kv head h, for RB * 16 query rows whose fragments are qf:
-// running maximum, sum (both for query row r16 of each block, the same in every lane group) and
-// output (lane: dims 16 dt + 4 kg + e of row r16). Returns whether a page id was outside the pool
-// (page 0 was read in its place).
-template <bool F16, int D, int RB>
-__device__ __forceinline__ bool attend(const AttnArgs& A, const int* table, int h, int k_lo, int k_hi, uint32_t lds,
-                                       int wv, int lane, const u32x4 (&qf)[RB][D / 32], float (&m)[RB], float (&l)[RB],
-                                       f32x4 (&o)[RB][D / 16]) {
-  typedef short v4s __attribute__((ext_vector_type(4)));
-  typedef __attribute__((address_space(3))) v4s lds_v4s;
-  typedef const __attribute__((address_space(3))) u32x4 lds_u32x4;
-  constexpr int CPR = D / 8, RPI = 64 / CPR, NI = KS / RPI;  // pieces a row, rows a DMA instruction, instructions
-  constexpr uint32_t VOFF = KS * D * 2;
-  const int r16 = lane & 15, kg = lane >> 4, pmask = (1 << A.lp) - 1;
-  const size_t page_elems = ((size_t)A.hkv << A.lp) * D, head_elems = ((size_t)h << A.lp) * D;
-  bool bad = false;
-  // page ids of 64 pages at a time, one a lane
-  int win0 = k_lo >> A.lp;
-  const int last_page = (k_hi - 1) >> A.lp;
-  typedef const __attribute__((address_space(1))) int gint;
-  int win = *(gint*)(table + min(win0 + lane, last_page));
-  auto page_id = [&](int at) {
-    if (at - win0 >= 64) {
-      win0 = at;
-      win = *(gint*)(table + min(win0 + lane, last_page));
+// The page ids of a run of keys, 64 at a time, one a lane; asked for in ascending order.
+struct Pages {
+  const int* table;
+  int first, last, ids, num_pages;
+  bool bad;  // an id was outside the pool (page 0 is read in its place)
+  __device__ __forceinline__ Pages(const int* t, int n, int page_lo, int page_last, int lane)
+      : table(t), first(page_lo), last(page_last), num_pages(n), bad(false) {
+    ids = *(gint*)(table + min(first + lane, last));
+  }
+  __device__ __forceinline__ int operator()(int page, int lane) {
+    if (page - first >= 64) {
+      first = page;
+      ids = *(gint*)(table + min(first + lane, last));
     }
-    const int id = __builtin_amdgcn_readlane(win, at - win0);
-    if (id >= 0 && id < A.num_pages) return id;
+    const int id = __builtin_amdgcn_readlane(ids, page - first);
+    if (id >= 0 && id < num_pages) return id;
     bad = true;
     return 0;
-  };
-  // the rows of the step at key k0 into stage s: K first, then V
-  auto fetch = [&](int k0, int s) {
-    const int at = k0 >> A.lp;
-    const size_t base0 = (size_t)page_id(at) * page_elems + head_elems;
-    // pages of 16 rows: the step's second half lies in the next page, if it has any key
-    const bool two = A.lp == 4 && k0 + 16 < k_hi;
-    const size_t base1 = two ? (size_t)page_id(at + 1) * page_elems + head_elems : base0;
-    const uint32_t dst = lds + s * stage_bytes<D>;
-#pragma unroll
-    for (int kv = 0; kv < 2; kv++) {
-      const uint16_t* pool = kv ? A.v : A.k;
-#pragma unroll
-      for (int i = 0; i < NI; i++) {
-        const int row = RPI * i + lane / CPR;
-        const int key = min(k0 + row, k_hi - 1);  // (rows past the end repeat the last key; their scores are masked)
-        const uint16_t* src = pool + (i * RPI < 16 ? base0 : base1) + (size_t)((key & pmask) * D + 8 * ((lane % CPR) ^ swz<D>(row)));
-        dma16(src, __builtin_amdgcn_readfirstlane(dst + kv * VOFF + 1024u * i));
-      }
-    }
-  };
-#pragma unroll
-  for (int rb = 0; rb < RB; rb++) {
-    m[rb] = -INFINITY;
-    l[rb] = 0.f;
-#pragma unroll
-    for (int dt = 0; dt < D / 16; dt++) o[rb][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  // fragment addresses in a stage: K row r16 (+ 16 t), pieces 4 ks + kg; V keys 4 kg + r16 / 4 (+ 16 t),
-  // dims 16 dt + 4 (r16 % 4) .. + 3
-  const uint32_t ka = r16 * (2 * D) + 16 * (kg ^ swz<D>(r16));
-  const int vrow = 4 * kg + (r16 >> 2);
-  const uint32_t va = VOFF + vrow * (2 * D) + 16 * (((r16 & 3) >> 1) ^ swz<D>(vrow)) + 8 * (r16 & 1);
-  const float c = A.scale_log2;
-  int k0 = k_lo + KS * wv, s = 0;
-  if (k0 < k_hi) fetch(k0, 0);
-  for (; k0 < k_hi; k0 += KS * AW, s ^= 1) {
-    const bool more = k0 + KS * AW < k_hi;
-    // the other stage's last reads are done before the DMA writes there
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (more) fetch(k0 + KS * AW, s ^ 1);
-    const uint32_t st = lds + s * stage_bytes<D>;
-    if (more) PG_AWAIT(3 * NI); else PG_AWAIT(NI);  // K is there
-    f32x4 sc[RB][2];
+};
+
+// 16 consecutive keys from k0 (a multiple of 16, so of one page) of K or V, to LDS: NI DMA
+// instructions. Rows past k_last repeat it, from its page `clamp` (their scores are masked, and a
+// row that is not there is never read).
+template <int D>
+__device__ __forceinline__ void fetch16(const uint16_t* pool, size_t base, int k0, int k_last, int pmask, uint32_t dst, int lane) {
+  constexpr int CPR = D / 8, RPI = 64 / CPR, NI = 16 / RPI;  // pieces a row, rows an instruction
 #pragma unroll
-    for (int t = 0; t < 2; t++) {
-      u32x4 kf[D / 32];
-#pragma unroll
-      for (int ks = 0; ks < D / 32; ks++) kf[ks] = *(lds_u32x4*)(uintptr_t)(st + ((ka ^ (64u * ks)) + 16u * 2 * D * t));
-#pragma unroll
-      for (int rb = 0; rb < RB; rb++) {
-        f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int ks = 0; ks < D / 32; ks++) a = mma<F16>(kf[ks], qf[rb][ks], a);
-#pragma unroll
-        for (int e = 0; e < 4; e++) a[e] *= c;
-        sc[rb][t] = a;
-      }
-    }
-    if (k0 + KS > k_hi) {
-#pragma unroll
-      for (int t = 0; t < 2; t++)
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-          if (k0 + 16 * t + 4 * kg + e >= k_hi)
-#pragma unroll
-            for (int rb = 0; rb < RB; rb++) sc[rb][t][e] = -INFINITY;
-    }
-    u32x4 pf[RB];
-#pragma unroll
-    for (int rb = 0; rb < RB; rb++) {
-      float mx = fmaxf(fmaxf(fmaxf(sc[rb][0][0], sc[rb][0][1]), fmaxf(sc[rb][0][2], sc[rb][0][3])),
-                       fmaxf(fmaxf(sc[rb][1][0], sc[rb][1][1]), fmaxf(sc[rb][1][2], sc[rb][1][3])));
-      mx = fmaxf(m[rb], groups_max(mx));
-      if (__any(mx > m[rb])) {  // (wave-uniform: a step that raises no maximum rescales nothing)
-        const float al = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rb] - mx);
-        l[rb] *= al;
-#pragma unroll
-        for (int dt = 0; dt < D / 16; dt++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) o[rb][dt][e] *= al;
-        m[rb] = mx;
-      }
-      const float base = m[rb] == -INFINITY ? 0.f : m[rb];
-      float p[8], sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        p[i] = __builtin_amdgcn_exp2f(sc[rb][i >> 2][i & 3] - base);
-        sum += p[i];
-      }
-      l[rb] += sum;  // (of this lane group's keys; joined after the last step)
-#pragma unroll
-      for (int i = 0; i < 4; i++) pf[rb][i] = pack2<F16>(p[2 * i], p[2 * i + 1]);
-    }
-    if (more) PG_AWAIT(2 * NI); else PG_AWAIT(0);  // V is there
-#pragma unroll
-    for (int dt = 0; dt < D / 16; dt++) {
-      const uint32_t a = st + (va ^ (32u * dt));
-      const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(uintptr_t)a));
-      const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(uintptr_t)(a + 16u * 2 * D)));
-      const u32x4 vf = u32x4{lo.x, lo.y, hi.x, hi.y};
-#pragma unroll
-      for (int rb = 0; rb < RB; rb++) o[rb][dt] = mma<F16>(vf, pf[rb], o[rb][dt]);
-    }
+  for (int i = 0; i < NI; i++) {
+    const int row = RPI * i + lane / CPR, key = min(k0 + row, k_last);
+    dma16(pool + base + (size_t)((key & pmask) * D + 8 * ((lane % CPR) ^ swz<D>(row))),
+          __builtin_amdgcn_readfirstlane(dst + 1024u * i));
   }
-#pragma unroll
-  for (int rb = 0; rb < RB; rb++) l[rb] = groups_sum(l[rb]);
-  return bad;
 }
 
-// One chunk of keys for RB * 16 query rows from row0 of `rows` rows of kv head h (row r: query head
-// h G + r % G of sequence b0 + r / G), to partial `slot`.
-template <bool F16, int D, int RB>
-__device__ void chunk(const AttnArgs& A, const int* table, int h, int b0, int row0, int rows, int k_lo, int k_hi, int slot,
-                      uint32_t lds, float (*s_m)[64], float (*s_l)[64]) {
-  typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
-  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, kg = lane >> 4;
-  u32x4 qf[RB][D / 32];
+// Fragment addresses in 16-key tiles of LDS rows: K row r16, pieces 4 ks + kg; V keys 4 kg + r16 / 4, dims
+// 16 dt + 4 (r16 % 4) .. + 3 (a tile t adds 32 t D bytes; ks and dt come in by XOR)
+template <int D>
+__device__ __forceinline__ uint32_t k_frag(int r16, int kg) { return r16 * (2 * D) + 16 * (kg ^ swz<D>(r16)); }
+template <int D>
+__device__ __forceinline__ uint32_t v_frag(int r16, int kg) {
+  const int row = 4 * kg + (r16 >> 2);
+  return row * (2 * D) + 16 * (((r16 & 3) >> 1) ^ swz<D>(row)) + 8 * (r16 & 1);
+}
+
+// One step of NT key tiles (K and V rows in LDS at kb and vb) for RB * 16 query rows: running maximum m and
+// sum l (of this lane group's keys) of query row r16 of each block, and output o (lane: dims 16 dt + 4 kg + e
+// of row r16). `left`: keys of the step that are there. before_v() runs between the scores and the
+// product with V.
+template <bool F16, int D, int RB, int NT, class BeforeV>
+__device__ __forceinline__ void attend_step(uint32_t kb, uint32_t vb, int left, float scale, int kg, uint32_t ka, uint32_t va,
+                                            const u32x4 (&qf)[RB][D / 32], float (&m)[RB], float (&l)[RB],
+                                            f32x4 (&o)[RB][D / 16], BeforeV before_v) {
+  f32x4 sc[RB][NT];
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    u32x4 kf[D / 32];
+#pragma unroll
+    for (int ks = 0; ks < D / 32; ks++) kf[ks] = *(lds_u32x4*)(uintptr_t)(kb + ((ka ^ (64u * ks)) + 32u * D * t));
+#pragma unroll
+    for (int rb = 0; rb < RB; rb++) {
+      f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < D / 32; ks++) a = mma<F16>(kf[ks], qf[rb][ks], a);
+      sc[rb][t] = a;
+    }
+  }
+  if (left < 16 * NT) {
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (16 * t + 4 * kg + e >= left)
+#pragma unroll
+          for (int rb = 0; rb < RB; rb++) sc[rb][t][e] = -INFINITY;
+  }
+  u32x4 pf[RB][NT / 2];
+#pragma unroll
+  for (int rb = 0; rb < RB; rb++) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < NT; t++) mx = fmaxf(fmaxf(fmaxf(sc[rb][t][0], sc[rb][t][1]), fmaxf(sc[rb][t][2], sc[rb][t][3])), mx);
+    mx = fmaxf(m[rb], groups_max(mx) * scale);
+    if (__any(mx > m[rb])) {  // (wave-uniform: a step that raises no maximum rescales nothing)
+      const float al = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rb] - mx);
+      l[rb] *= al;
+#pragma unroll
+      for (int dt = 0; dt < D / 16; dt++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[rb][dt][e] *= al;
+      m[rb] = mx;
+    }
+    const float base = m[rb] == -INFINITY ? 0.f : m[rb];
+    float sum = 0.f;
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      float p[4];
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        p[e] = __builtin_amdgcn_exp2f(fmaf(sc[rb][t][e], scale, -base));
+        sum += p[e];
+      }
+      pf[rb][t / 2][2 * (t % 2)] = pack2<F16>(p[0], p[1]);
+      pf[rb][t / 2][2 * (t % 2) + 1] = pack2<F16>(p[2], p[3]);
+    }
+    l[rb] += sum;
+  }
+  before_v();
+#pragma unroll
+  for (int j = 0; j < NT / 2; j++)
+#pragma unroll
+    for (int dt = 0; dt < D / 16; dt++) {
+      const uint32_t a = vb + (va ^ (32u * dt)) + 64u * D * j;
+      const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(uintptr_t)a));
+      const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(uintptr_t)(a + 32u * D)));
+      const u32x4 vf = u32x4{lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+      for (int rb = 0; rb < RB; rb++) o[rb][dt] = mma<F16>(vf, pf[rb][j], o[rb][dt]);
+    }
+}
+
+// Query fragments of rows row0 + 16 rb + r16 (row r of a kv head: its query r % G of sequence b0 + r / G)
+template <int D, int RB>
+__device__ __forceinline__ void load_q(const AttnArgs& A, int h, int b0, int row0, int rows, int r16, int kg,
+                                       u32x4 (&qf)[RB][D / 32]) {
 #pragma unroll
   for (int rb = 0; rb < RB; rb++) {
     const int r = min(row0 + 16 * rb + r16, rows - 1);  // (rows past the end repeat the last one and are not stored)
@@ -391,20 +375,90 @@ __device__ void chunk(const AttnArgs& A, const int* table, int h, int b0, int ro
 #pragma unroll
     for (int ks = 0; ks < D / 32; ks++) qf[rb][ks] = *(gu32x4*)(q + 32 * ks + 8 * kg);
   }
+}
+
+// Where row r's result goes: part `slot` of the partial results, or, as the only part, the output.
+template <bool F16, int D>
+__device__ __forceinline__ void store_o(const AttnArgs& A, int slot, int h, int b0, int r, int d0, f32x4 x, float m, float l) {
+  const int b = b0 + r / A.g, hq = h * A.g + r % A.g;
+  if (A.np + A.ns == 1) {
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    *reinterpret_cast<u32x2*>(A.out + (size_t)b * A.o_sb + (size_t)hq * A.o_sh + d0) =
+        u32x2{pack2<F16>(x[0] * inv, x[1] * inv), pack2<F16>(x[2] * inv, x[3] * inv)};
+    return;
+  }
+  const size_t at = ((size_t)slot * A.batch + b) * A.hq + hq;
+  *reinterpret_cast<f32x4*>(A.part_o + at * D + d0) = x;
+  if (d0 == 0) A.part_ml[at] = make_float2(m, l);
+}
+
+// Keys [k_lo, k_hi) of `table` for up to RB * 16 query rows. The waves take 32-key steps in turn and do not
+// wait for each other until the end: each has 16 KB of LDS, half for K and half for V, and asks for the next
+// step's K as soon as it has the scores of this one, for its V once this one's is multiplied.
+template <bool F16, int D, int RB>
+__device__ __forceinline__ void own_part(const AttnArgs& A, const int* table, int h, int b0, int row0, int rows, int k_lo, int k_hi,
+                                         int slot, uint32_t lds, float (*s_m)[64], float (*s_l)[64]) {
+  constexpr uint32_t HALF = KS * D * 2, WAVE = 2 * HALF;  // bytes of a step's K (or V), and of a wave
+  constexpr int NI = KS * D * 2 / 1024;                   // DMA instructions of a step's K (or V)
+  static_assert(RB * 16 * D * 4 <= (int)WAVE, "a wave's output fits its LDS");
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, kg = lane >> 4;
+  const int pmask = (1 << A.lp) - 1;
+  const size_t page_elems = ((size_t)A.hkv << A.lp) * D, head_elems = ((size_t)h << A.lp) * D;
+  const uint32_t mine = lds + WAVE * wv;
+  Pages pages(table, A.num_pages, k_lo >> A.lp, (k_hi - 1) >> A.lp, lane);
+  size_t base[2];  // the pages of a step's two 16-key halves
+  auto find = [&](int k0) {
+    base[0] = (size_t)pages(k0 >> A.lp, lane) * page_elems + head_elems;
+    base[1] = A.lp == 4 && k0 + 16 < k_hi ? (size_t)pages((k0 >> 4) + 1, lane) * page_elems + head_elems : base[0];
+  };
+  auto fetch = [&](const uint16_t* pool, int k0, uint32_t dst) {
+    fetch16<D>(pool, base[0], k0, k_hi - 1, pmask, dst, lane);
+    fetch16<D>(pool, base[1], k0 + 16, k_hi - 1, pmask, dst + HALF / 2, lane);
+  };
+  int k0 = k_lo + KS * wv;
+  if (k0 < k_hi) {
+    find(k0);
+    fetch(A.k, k0, mine);
+    fetch(A.v, k0, mine + HALF);
+  }
+  u32x4 qf[RB][D / 32];
+  load_q<D, RB>(A, h, b0, row0, rows, r16, kg, qf);
   float m[RB], l[RB];
   f32x4 o[RB][D / 16];
-  constexpr uint32_t WAVE = STAGES * stage_bytes<D>;
-  static_assert(RB * 16 * D * 4 <= (int)WAVE, "a wave's output fits its stages");
-  const uint32_t mine = lds + WAVE * wv;
-  const bool bad = attend<F16, D, RB>(A, table, h, k_lo, k_hi, mine, wv, lane, qf, m, l, o);
-  // ---- join the waves: each scales its output to the rows' common maximum and leaves it in its stages
-  // (row: D / 4 pieces of 16 bytes, swizzled with the row), then all add the four up
-  if (kg == 0)
 #pragma unroll
-    for (int rb = 0; rb < RB; rb++) {
+  for (int rb = 0; rb < RB; rb++) {
+    m[rb] = -INFINITY;
+    l[rb] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < D / 16; dt++) o[rb][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const uint32_t ka = k_frag<D>(r16, kg), va = v_frag<D>(r16, kg);
+  for (; k0 < k_hi; k0 += KS * AW) {
+    const int next = k0 + KS * AW;
+    PG_AWAIT(NI);  // K is there (V may be in flight)
+    attend_step<F16, D, RB, KS / 16>(mine, mine + HALF, k_hi - k0, A.scale_log2, kg, ka, va, qf, m, l, o, [&] {
+      PG_READ();  // (K is in registers)
+      if (next < k_hi) {
+        find(next);
+        fetch(A.k, next, mine);
+        PG_AWAIT(NI);  // V is there (the next K may be in flight)
+      } else {
+        PG_AWAIT(0);
+      }
+    });
+    PG_READ();
+    if (next < k_hi) fetch(A.v, next, mine + HALF);
+  }
+  // ---- join the waves: each scales its output to the rows' common maximum and leaves it in its LDS (row:
+  // D / 4 pieces of 16 bytes, swizzled with the row), then all add the four up
+#pragma unroll
+  for (int rb = 0; rb < RB; rb++) {
+    l[rb] = groups_sum(l[rb]);
+    if (kg == 0) {
       s_m[wv][16 * rb + r16] = m[rb];
-      s_l[wv][16 * rb + r16] = bad ? NAN : l[rb];
+      s_l[wv][16 * rb + r16] = pages.bad ? NAN : l[rb];
     }
+  }
   __syncthreads();
 #pragma unroll
   for (int rb = 0; rb < RB; rb++) {
@@ -423,55 +477,99 @@ __device__ void chunk(const AttnArgs& A, const int* table, int h, int b0, int ro
   }
   __syncthreads();
   constexpr int PPR = D / 4;  // 16-byte pieces a row
-  for (int i = tid; i < RB * 16 * PPR; i += 64 * AW) {
-    const int r = i / PPR, p = i % PPR, row = row0 + r;
-    if (row >= rows) break;
+  const int n = min(RB * 16, rows - row0) * PPR;
+  for (int i = tid; i < n; i += 64 * AW) {
+    const int r = i / PPR, p = i % PPR;
     f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < AW; w++) x += *(lds_f32x4*)(uintptr_t)(lds + WAVE * w + r * (4 * D) + 16 * (p ^ (r & 15)));
-    const size_t at = (size_t)slot * A.batch * A.hq + (size_t)(b0 + row / A.g) * A.hq + h * A.g + row % A.g;
-    *reinterpret_cast<f32x4*>(A.part_o + at * D + 4 * p) = x;
-    if (p == 0) {
-      float mx = s_m[0][r], sum = 0.f;
+    float mx = s_m[0][r], sum = 0.f;
 #pragma unroll
-      for (int w = 1; w < AW; w++) mx = fmaxf(mx, s_m[w][r]);
+    for (int w = 1; w < AW; w++) mx = fmaxf(mx, s_m[w][r]);
 #pragma unroll
-      for (int w = 0; w < AW; w++) {
-        const float mw = s_m[w][r];
-        sum += s_l[w][r] * (mw == -INFINITY ? (s_l[w][r] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(mw - mx));
-      }
-      A.part_ml[at] = make_float2(mx, sum);
+    for (int w = 0; w < AW; w++) {
+      const float mw = s_m[w][r], lw = s_l[w][r];
+      sum += lw == 0.f ? 0.f : lw * __builtin_amdgcn_exp2f(mw - (mx == -INFINITY ? 0.f : mx));
     }
+    store_o<F16, D>(A, slot, h, b0, row0 + r, 4 * p, x, mx, sum);
   }
 }
 
-// keys of one part of `parts` of `len` keys, in whole steps of the workgroup's four waves
-__device__ __forceinline__ int part_keys(int len, int parts) {
-  constexpr int U = KS * AW;
-  return ((len + parts - 1) / parts + U - 1) / U * U;
+// Keys [k_lo, k_hi) of the prefix for up to 64 RB query rows from row0 of all `rows`: wave w takes RB blocks
+// of 16 rows from row0 + 16 RB w and all the keys, 64 at a time, from LDS that the workgroup fills together
+// (two stages: the next one is on its way while this one is multiplied). One barrier a step: once every
+// wave is there, the stage is complete and the other one has been read.
+template <bool F16, int D, int RB>
+__device__ __forceinline__ void prefix_part(const AttnArgs& A, int h, int row0, int rows, int k_lo, int k_hi, int slot, uint32_t lds) {
+  constexpr uint32_t HALF = TS * D * 2, STAGE = 2 * HALF;
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, kg = lane >> 4;
+  const int pmask = (1 << A.lp) - 1;
+  const size_t page_elems = ((size_t)A.hkv << A.lp) * D, head_elems = ((size_t)h << A.lp) * D;
+  Pages pages(A.prefix_pages, A.num_pages, k_lo >> A.lp, (k_hi - 1) >> A.lp, lane);
+  // wave w brings keys 16 w .. + 15 of a step; a step's first page past the end is its last key's
+  auto fetch = [&](int k0, uint32_t dst) {
+    const int k = min(k0 + 16 * wv, k_hi - 1);
+    const size_t base = (size_t)pages(k >> A.lp, lane) * page_elems + head_elems;
+    fetch16<D>(A.k, base, k0 + 16 * wv, k_hi - 1, pmask, dst + HALF / 4 * wv, lane);
+    fetch16<D>(A.v, base, k0 + 16 * wv, k_hi - 1, pmask, dst + HALF + HALF / 4 * wv, lane);
+  };
+  fetch(k_lo, lds);
+  u32x4 qf[RB][D / 32];
+  const int mine = row0 + 16 * RB * wv;
+  load_q<D, RB>(A, h, 0, mine, rows, r16, kg, qf);
+  float m[RB], l[RB];
+  f32x4 o[RB][D / 16];
+#pragma unroll
+  for (int rb = 0; rb < RB; rb++) {
+    m[rb] = -INFINITY;
+    l[rb] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < D / 16; dt++) o[rb][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const uint32_t ka = k_frag<D>(r16, kg), va = v_frag<D>(r16, kg);
+  uint32_t st = 0;
+  for (int k0 = k_lo; k0 < k_hi; k0 += TS, st ^= STAGE) {
+    PG_BARRIER();
+    if (k0 + TS < k_hi) fetch(k0 + TS, lds + (st ^ STAGE));
+    attend_step<F16, D, RB, TS / 16>(lds + st, lds + st + HALF, k_hi - k0, A.scale_log2, kg, ka, va, qf, m, l, o, [] {});
+  }
+  // every wave has seen some of the page ids: a bad one anywhere reaches all rows of the tile
+  const int bad = __syncthreads_or(pages.bad);
+#pragma unroll
+  for (int rb = 0; rb < RB; rb++) {
+    const int r = mine + 16 * rb + r16;
+    const float sum = bad ? NAN : groups_sum(l[rb]);
+    if (r < rows)
+#pragma unroll
+      for (int dt = 0; dt < D / 16; dt++) store_o<F16, D>(A, slot, h, 0, r, 16 * dt + 4 * kg, o[rb][dt], m[rb], sum);
+  }
 }
 
-template <bool F16, int D, int RB>
-__global__ void __launch_bounds__(64 * AW) attn_kernel(AttnArgs A) {
-  __shared__ __align__(1024) uint8_t s_kv[AW * STAGES * stage_bytes<D>];
+// keys of one part of `parts` of `len` keys, in units of 128 (a step for each wave, two of the prefix)
+constexpr int UNIT = KS * AW;
+__host__ __device__ __forceinline__ int part_keys(int len, int parts) { return ((len + parts - 1) / parts + UNIT - 1) / UNIT * UNIT; }
+
+// How the query rows of a prefix are tiled: up to 32 rows, all keys' work is split among the waves (own_part);
+// more rows are (prefix_part).
+enum : int { ROWS16 = 0, ROWS32 = 1, ROWS64 = 2, ROWS128 = 3 };
+__host__ __device__ constexpr int tile_rows(int form) { return 16 << form; }
+
+template <bool F16, int D, int FORM>
+__global__ void __launch_bounds__(64 * AW, 2) attn_kernel(AttnArgs A) {
+  __shared__ __align__(1024) uint8_t s_kv[4 * TS * D * 2];
   __shared__ float s_m[AW][64], s_l[AW][64];
+  static_assert(sizeof(s_kv) == AW * 2 * KS * D * 2, "the two forms take the same LDS");
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&s_kv[0];
   int id = blockIdx.x;
   const int h = id % A.hkv;  // (fastest: with 8 kv heads each XCD reads one head's rows)
   id /= A.hkv;
   if (id < A.prefix_tiles * A.np) {
-    const int tile = id % A.prefix_tiles, part = id / A.prefix_tiles;
+    const int rows = A.batch * A.g, row0 = tile_rows(FORM) * (id % A.prefix_tiles), part = id / A.prefix_tiles;
     const int ch = part_keys(A.prefix_len, A.np), lo = part * ch, hi = min(A.prefix_len, lo + ch);
-    if (lo >= hi) {
-      // (the last parts of a prefix that does not fill them all)
-      for (int r = threadIdx.x; r < 16 * RB; r += 64 * AW) {
-        const int row = 16 * RB * tile + r;
-        if (row < A.batch * A.g)
-          A.part_ml[(size_t)part * A.batch * A.hq + (size_t)(row / A.g) * A.hq + h * A.g + row % A.g] = make_float2(-INFINITY, 0.f);
-      }
-      return;
-    }
-    chunk<F16, D, RB>(A, A.prefix_pages, h, 0, 16 * RB * tile, A.batch * A.g, lo, hi, part, lds, s_m, s_l);
+    if constexpr (FORM <= ROWS32)
+      own_part<F16, D, FORM == ROWS16 ? 1 : 2>(A, A.prefix_pages, h, 0, row0, rows, lo, hi, part, lds, s_m, s_l);
+    else
+      prefix_part<F16, D, FORM == ROWS64 ? 1 : 2>(A, h, row0, rows, lo, hi, part, lds);
     return;
   }
   id -= A.prefix_tiles * A.np;
@@ -481,52 +579,69 @@ __global__ void __launch_bounds__(64 * AW) attn_kernel(AttnArgs A) {
   const int len = max(0, min(A.lens[b] + A.len_add, A.width << A.lp));
   const int ch = part_keys(len, A.ns), lo = part * ch, hi = min(len, lo + ch);
   if (lo >= hi) {
-    const int r = 16 * tile + threadIdx.x;
-    if (threadIdx.x < 16 && r < A.g)
-      A.part_ml[(size_t)(A.np + part) * A.batch * A.hq + (size_t)b * A.hq + h * A.g + r] = make_float2(-INFINITY, 0.f);
+    // no key: the part's sum says so, or, as the only part, the output is zero
+    const int n = min(16, A.g - 16 * tile) * (D / 4);
+    for (int i = threadIdx.x; i < n; i += 64 * AW)
+      if (A.np + A.ns == 1 || i % (D / 4) == 0)
+        store_o<F16, D>(A, A.np + part, h, b, 16 * tile + i / (D / 4), 4 * (i % (D / 4)), f32x4{0.f, 0.f, 0.f, 0.f}, -INFINITY, 0.f);
     return;
   }
-  chunk<F16, D, 1>(A, A.tables + (size_t)b * A.t_sb + (size_t)h * A.t_sh, h, b, 16 * tile, A.g, lo, hi, A.np + part, lds, s_m,
-                   s_l);
+  own_part<F16, D, 1>(A, A.tables + (size_t)b * A.t_sb + (size_t)h * A.t_sh, h, b, 16 * tile, A.g, lo, hi, A.np + part, lds, s_m,
+                      s_l);
 }
 
-// Workgroup (query head, sequence): the parts' outputs, scaled to their common maximum, over their
-// sums. Rows without a key give zeros. Eight (D = 128) or sixteen groups of lanes take the parts in
-// turn; the groups are added in order, so a result does not depend on timing.
+// A wave a row (query head, sequence): the parts' outputs, scaled to their common maximum, over their sums.
+// Rows without a key give zeros. Lane p takes part p's maximum and sum (and part p + 64's); LPR lanes hold
+// a row's output, and the wave's 64 / LPR groups of them take the parts in turn, eight in flight, and are
+// added in order, so that a result does not depend on timing.
+constexpr int MAX_PARTS = 128;
 template <bool F16, int D>
 __global__ void __launch_bounds__(256) combine_kernel(AttnArgs A) {
-  constexpr int LPR = D / 4, GROUPS = 256 / LPR;
-  __shared__ f32x4 s_o[GROUPS][LPR];
-  __shared__ float s_l[GROUPS];
-  const int hq = blockIdx.x, b = blockIdx.y, parts = A.np + A.ns, lane = threadIdx.x % LPR, grp = threadIdx.x / LPR;
-  const size_t row = (size_t)b * A.hq + hq, step = (size_t)A.batch * A.hq;
-  float mx = -INFINITY;
-  for (int p = 0; p < parts; p++) mx = fmaxf(mx, A.part_ml[row + step * p].x);
-  const float base = mx == -INFINITY ? 0.f : mx;
-  f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
-  float l = 0.f;
-  for (int p = grp; p < parts; p += GROUPS) {
-    const float2 ml = A.part_ml[row + step * p];
-    if (ml.y == 0.f) continue;  // (no key: its output was not written)
-    const float w = __builtin_amdgcn_exp2f(ml.x - base);
-    const f32x4 y = *reinterpret_cast<const f32x4*>(A.part_o + (row + step * p) * D + 4 * lane);
-    l += w * ml.y;
+  constexpr int LPR = D / 4, GROUPS = 64 / LPR, AHEAD = 8;
+  const int lane = threadIdx.x & 63, parts = A.np + A.ns;
+  const size_t rows = (size_t)A.batch * A.hq, row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const int grp = lane / LPR, c = lane % LPR;
+  float2 ml[2];
 #pragma unroll
-    for (int e = 0; e < 4; e++) x[e] += w * y[e];
+  for (int i = 0; i < 2; i++) ml[i] = lane + 64 * i < parts ? A.part_ml[row + rows * (lane + 64 * i)] : make_float2(-INFINITY, 0.f);
+  float mx[1] = {fmaxf(ml[0].x, ml[1].x)};
+  wave_max_n(mx);
+  const float base = mx[0] == -INFINITY ? 0.f : mx[0];
+  float w[2], l = 0.f;
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const float f = __builtin_amdgcn_exp2f(ml[i].x - base);
+    l += ml[i].y == 0.f ? 0.f : f * ml[i].y;
+    w[i] = ml[i].y == 0.f ? -1.f : f;  // (no key: its output was not written)
   }
-  s_o[grp][lane] = x;
-  if (lane == 0) s_l[grp] = l;
-  __syncthreads();
+  l = wave_sum(l);
+  f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int p0 = 0; p0 < parts; p0 += GROUPS * AHEAD) {
+    f32x4 y[AHEAD];
+    float f[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; u++) {
+      const int p = p0 + GROUPS * u + grp;
+      f[u] = __shfl(p < 64 ? w[0] : w[1], p & 63, 64);
+      if (p >= parts) f[u] = -1.f;
+      y[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (f[u] >= 0.f || f[u] != f[u]) y[u] = *reinterpret_cast<const f32x4*>(A.part_o + (row + rows * p) * D + 4 * c);
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; u++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[e] += f[u] * y[u][e];
+  }
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    if (GROUPS == 4) x[e] += __shfl_xor(x[e], 16, 64);
+    x[e] += __shfl_xor(x[e], 32, 64);
+  }
   if (grp > 0) return;
-  for (int g = 1; g < GROUPS; g++) {
-    x += s_o[g][lane];
-    l += s_l[g];
-  }
   const float inv = l == 0.f ? 0.f : 1.0f / l;
-  u32x2 w;
-  w.x = pack2<F16>(x[0] * inv, x[1] * inv);
-  w.y = pack2<F16>(x[2] * inv, x[3] * inv);
-  *reinterpret_cast<u32x2*>(A.out + (size_t)b * A.o_sb + (size_t)hq * A.o_sh + 4 * lane) = w;
+  *reinterpret_cast<u32x2*>(A.out + row / A.hq * A.o_sb + row % A.hq * A.o_sh + 4 * c) =
+      u32x2{pack2<F16>(x[0] * inv, x[1] * inv), pack2<F16>(x[2] * inv, x[3] * inv)};
 }
 
 // ------------------------------------------------------------------ choosing pages
@@ -750,43 +865,45 @@ int append_rows(const AppendArgs& A, bool f16, hipStream_t stream) {
   return hipGetLastError() == hipSuccess ? MQ_OK : MQ_ERR_HIP;
 }
 
-// How an attention call is split. Query rows of the prefix go in tiles of 16, 32 or 64, so that its
-// keys are read as few times as there are tiles; a sequence's own rows are shared by its G query
-// heads a kv head only, in tiles of 16. Keys are split until the launch has about two workgroups a
-// CU (one is resident, the next follows), in parts of at least 128 keys (a step for each wave).
+// How an attention call is split. Query rows of the prefix go in tiles of up to 128, so that its keys are read
+// as few times as there are tiles; a sequence's own rows are shared by its G query heads a kv head only, in
+// tiles of 16. Keys are split until the launch has about two workgroups a CU, in parts of at least 128 keys.
 AttnPlan plan_attention(int batch, int hkv, int g, int d, int prefix_len, int max_len) {
   AttnPlan p{};
-  constexpr int UNIT = KS * AW, WANT = 512, MAX_PARTS = 64;
+  constexpr int WANT = 512;
   const int rows = batch * g;
-  p.rb = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  p.form = rows <= 16 ? ROWS16 : rows <= 32 ? ROWS32 : rows <= 64 ? ROWS64 : ROWS128;
   p.own_tiles = (g + 15) / 16;
   auto parts = [&](int len, long long tiles) {
     const int most = (len + UNIT - 1) / UNIT;
     long long n = (WANT + tiles - 1) / tiles;
     if (n > most) n = most;
-    return (int)(n > MAX_PARTS ? MAX_PARTS : n);
+    if (n > MAX_PARTS / 2) n = MAX_PARTS / 2;
+    const int ch = part_keys(len, (int)n);
+    return (len + ch - 1) / ch;  // (as many as have a key)
   };
   if (prefix_len > 0) {
-    p.prefix_tiles = (rows + 16 * p.rb - 1) / (16 * p.rb);
+    p.prefix_tiles = (rows + tile_rows(p.form) - 1) / tile_rows(p.form);
     p.np = parts(prefix_len, (long long)hkv * p.prefix_tiles);
   }
   if (max_len > 0) p.ns = parts(max_len, (long long)batch * hkv * p.own_tiles);
-  const size_t rows_all = (size_t)(p.np + p.ns) * batch * hkv * g;
+  const size_t rows_all = p.np + p.ns == 1 ? 0 : (size_t)(p.np + p.ns) * batch * hkv * g;
   p.out_bytes = (rows_all * d * 4 + 255) / 256 * 256;
   p.bytes = p.out_bytes + (rows_all * 8 + 255) / 256 * 256;
   return p;
 }
 
 template <bool F16, int D>
-static void attn_launch(const AttnArgs& A, int rb, unsigned blocks, hipStream_t stream) {
+static void attn_launch(const AttnArgs& A, int form, unsigned blocks, hipStream_t stream) {
   if (blocks > 0) {
-    switch (rb) {
-      case 1: attn_kernel<F16, D, 1><<<blocks, 64 * AW, 0, stream>>>(A); break;
-      case 2: attn_kernel<F16, D, 2><<<blocks, 64 * AW, 0, stream>>>(A); break;
-      default: attn_kernel<F16, D, 4><<<blocks, 64 * AW, 0, stream>>>(A); break;
+    switch (form) {
+      case ROWS16: attn_kernel<F16, D, ROWS16><<<blocks, 64 * AW, 0, stream>>>(A); break;
+      case ROWS32: attn_kernel<F16, D, ROWS32><<<blocks, 64 * AW, 0, stream>>>(A); break;
+      case ROWS64: attn_kernel<F16, D, ROWS64><<<blocks, 64 * AW, 0, stream>>>(A); break;
+      default: attn_kernel<F16, D, ROWS128><<<blocks, 64 * AW, 0, stream>>>(A); break;
     }
   }
-  combine_kernel<F16, D><<<dim3(A.hq, A.batch), 256, 0, stream>>>(A);
+  if (A.np + A.ns != 1) combine_kernel<F16, D><<<((unsigned)A.batch * A.hq + 3) / 4, 256, 0, stream>>>(A);
 }
 
 // Both launches of an attention; A without its split and partial results, which come from `p` and
@@ -798,9 +915,9 @@ int run_attention(AttnArgs A, const AttnPlan& p, int d, bool f16, void* ws, hipS
   const long long blocks = (long long)A.hkv * ((long long)p.prefix_tiles * p.np + (long long)p.own_tiles * A.batch * p.ns);
   if (blocks > 0x7fffffff) return MQ_ERR_ARG;
   if (d == 128)
-    f16 ? attn_launch<true, 128>(A, p.rb, (unsigned)blocks, stream) : attn_launch<false, 128>(A, p.rb, (unsigned)blocks, stream);
+    f16 ? attn_launch<true, 128>(A, p.form, (unsigned)blocks, stream) : attn_launch<false, 128>(A, p.form, (unsigned)blocks, stream);
   else
-    f16 ? attn_launch<true, 64>(A, p.rb, (unsigned)blocks, stream) : attn_launch<false, 64>(A, p.rb, (unsigned)blocks, stream);
+    f16 ? attn_launch<true, 64>(A, p.form, (unsigned)blocks, stream) : attn_launch<false, 64>(A, p.form, (unsigned)blocks, stream);
   return hipGetLastError() == hipSuccess ? MQ_OK : MQ_ERR_HIP;
 }
 
@@ -811,7 +928,7 @@ static bool attn_ok(const MqPagePool* P, bool sparse, const void* q, int64_t q_s
                     int64_t o_sh, int num_q_heads, int batch, const int* tables, int64_t t_sb, int width, const int* lens,
                     float scale, const void* ws) {
   return pool_ok(P, sparse) && rows_ok(q, q_sb, q_sh) && rows_ok(out, o_sb, o_sh) && batch >= 1 && batch <= 65535 &&
-         num_q_heads >= P->num_kv_heads && num_q_heads <= 65535 && num_q_heads % P->num_kv_heads == 0 && tables && lens &&
+         num_q_heads >= P->num_kv_heads && num_q_heads <= 16384 && num_q_heads % P->num_kv_heads == 0 && tables && lens &&
          width >= 1 && width <= MQ_MAX_TABLE_WIDTH && t_sb >= 0 && scale > 0.f && isfinite(scale) && ws && aligned16(ws);
 }
 
