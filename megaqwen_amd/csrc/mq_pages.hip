@@ -192,6 +192,7 @@ __global__ void __launch_bounds__(CT) append_kernel(AppendArgs A) {
 // operand of O^T = V^T P^T, whose V^T comes from LDS by transpose reads in the same key order. The
 // probabilities are rounded to 16 bits for that product (a relative 2^-9 (bf16) of each term, as
 // much as the output's own rounding); maxima, sums and outputs stay in 32 bits.
+constexpr int NUM_CUS = 256;
 constexpr int AW = 4;   // waves
 constexpr int KS = 32;  // keys a wave takes at a time, of own rows
 constexpr int TS = 64;  // keys a workgroup takes at a time, of a prefix whose rows its waves share out
@@ -218,18 +219,15 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   else
     return pack_bf2(lo, hi);
 }
-// maximum and sum over the four 16-lane groups (lanes l, l + 16, l + 32, l + 48), in every group
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
+}
+// maximum over the four 16-lane groups (lanes l, l + 16, l + 32, l + 48), in every group
 __device__ __forceinline__ float groups_max(float v) {
   const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
   const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ __forceinline__ float groups_sum(float v) {
-  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
 typedef short v4s __attribute__((ext_vector_type(4)));
@@ -288,13 +286,22 @@ __device__ __forceinline__ uint32_t v_frag(int r16, int kg) {
   return row * (2 * D) + 16 * (((r16 & 3) >> 1) ^ swz<D>(row)) + 8 * (r16 & 1);
 }
 
-// One step of NT key tiles (K and V rows in LDS at kb and vb) for RB * 16 query rows: running maximum m and
-// sum l (of this lane group's keys) of query row r16 of each block, and output o (lane: dims 16 dt + 4 kg + e
-// of row r16). `left`: keys of the step that are there. before_v() runs between the scores and the
-// product with V.
+// m is the maximum that a row's probabilities are taken relative to; it follows the true one once that is
+// 2^SLACK times as large as it, so that few steps have to rescale l and o (their 64 products a 64-key step were
+// 40% of all vector instructions: with each new maximum of any of 16 rows, 51 us for the prefix of 15001
+// rows and 512 queries). Probabilities reach 2^SLACK then, which no type here minds.
+constexpr float SLACK = 8.f;
+
+// One step of NT key tiles (K and V rows in LDS at kb and vb) for RB * 16 query rows: running maximum m of
+// query row r16 of each block, sum l (four equal values) and output o (lane: dims 16 dt + 4 kg + e of row r16).
+// `left`: keys of the step that are there. before_v() runs between the scores and the product with V.
+// The vector units are the tighter bound here (two products a score pair cost the matrix units 1024 cycles a
+// 64-key step of 32 rows), so the sum of the probabilities is another row of the product, with ones
+// for V, and the maximum takes three operands (v_maximum3_f32; a score that is not a number
+// makes its row's output not a number either way).
 template <bool F16, int D, int RB, int NT, class BeforeV>
 __device__ __forceinline__ void attend_step(uint32_t kb, uint32_t vb, int left, float scale, int kg, uint32_t ka, uint32_t va,
-                                            const u32x4 (&qf)[RB][D / 32], float (&m)[RB], float (&l)[RB],
+                                            const u32x4 (&qf)[RB][D / 32], float (&m)[RB], f32x4 (&l)[RB],
                                             f32x4 (&o)[RB][D / 16], BeforeV before_v) {
   f32x4 sc[RB][NT];
 #pragma unroll
@@ -311,6 +318,7 @@ __device__ __forceinline__ void attend_step(uint32_t kb, uint32_t vb, int left, 
     }
   }
   if (left < 16 * NT) {
+    asm volatile("");  // (a branch: as selects it would cost every step)
 #pragma unroll
     for (int t = 0; t < NT; t++)
 #pragma unroll
@@ -319,40 +327,51 @@ __device__ __forceinline__ void attend_step(uint32_t kb, uint32_t vb, int left, 
 #pragma unroll
           for (int rb = 0; rb < RB; rb++) sc[rb][t][e] = -INFINITY;
   }
-  u32x4 pf[RB][NT / 2];
+  float mx[RB];
+  bool raise = false;
 #pragma unroll
   for (int rb = 0; rb < RB; rb++) {
-    float mx = -INFINITY;
+    mx[rb] = -INFINITY;
 #pragma unroll
-    for (int t = 0; t < NT; t++) mx = fmaxf(fmaxf(fmaxf(sc[rb][t][0], sc[rb][t][1]), fmaxf(sc[rb][t][2], sc[rb][t][3])), mx);
-    mx = fmaxf(m[rb], groups_max(mx) * scale);
-    if (__any(mx > m[rb])) {  // (wave-uniform: a step that raises no maximum rescales nothing)
-      const float al = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rb] - mx);
-      l[rb] *= al;
+    for (int t = 0; t < NT; t++)
+      mx[rb] = max3(max3(mx[rb], sc[rb][t][0], sc[rb][t][1]), sc[rb][t][2], sc[rb][t][3]);
+    mx[rb] = fmaxf(m[rb], groups_max(mx[rb]) * scale);
+    raise |= mx[rb] > m[rb] + SLACK;
+  }
+  if (__any(raise)) {
+#pragma unroll
+    for (int rb = 0; rb < RB; rb++) {
+      const float al = mx[rb] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rb] - mx[rb]);
+#pragma unroll
+      for (int e = 0; e < 4; e++) l[rb][e] *= al;
 #pragma unroll
       for (int dt = 0; dt < D / 16; dt++)
 #pragma unroll
         for (int e = 0; e < 4; e++) o[rb][dt][e] *= al;
-      m[rb] = mx;
+      m[rb] = mx[rb];
     }
-    const float base = m[rb] == -INFINITY ? 0.f : m[rb];
-    float sum = 0.f;
-#pragma unroll
-    for (int t = 0; t < NT; t++) {
-      float p[4];
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        p[e] = __builtin_amdgcn_exp2f(fmaf(sc[rb][t][e], scale, -base));
-        sum += p[e];
-      }
-      pf[rb][t / 2][2 * (t % 2)] = pack2<F16>(p[0], p[1]);
-      pf[rb][t / 2][2 * (t % 2) + 1] = pack2<F16>(p[2], p[3]);
-    }
-    l[rb] += sum;
   }
   before_v();
+  constexpr uint32_t ONE = F16 ? 0x3c003c00u : 0x3f803f80u;
+  const u32x4 ones = u32x4{ONE, ONE, ONE, ONE};
+  // (straight-line from here: the exponentials of one 32-key half run beside the products of the other)
 #pragma unroll
-  for (int j = 0; j < NT / 2; j++)
+  for (int j = 0; j < NT / 2; j++) {
+    u32x4 pf[RB];
+#pragma unroll
+    for (int rb = 0; rb < RB; rb++) {
+      const float base = m[rb] == -INFINITY ? 0.f : m[rb];
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) p[e] = __builtin_amdgcn_exp2f(fmaf(sc[rb][2 * j + t][e], scale, -base));
+        pf[rb][2 * t] = pack2<F16>(p[0], p[1]);
+        pf[rb][2 * t + 1] = pack2<F16>(p[2], p[3]);
+      }
+    }
+#pragma unroll
+    for (int rb = 0; rb < RB; rb++) l[rb] = mma<F16>(ones, pf[rb], l[rb]);
 #pragma unroll
     for (int dt = 0; dt < D / 16; dt++) {
       const uint32_t a = vb + (va ^ (32u * dt)) + 64u * D * j;
@@ -360,8 +379,9 @@ __device__ __forceinline__ void attend_step(uint32_t kb, uint32_t vb, int left, 
       const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(uintptr_t)(a + 32u * D)));
       const u32x4 vf = u32x4{lo.x, lo.y, hi.x, hi.y};
 #pragma unroll
-      for (int rb = 0; rb < RB; rb++) o[rb][dt] = mma<F16>(vf, pf[rb][j], o[rb][dt]);
+      for (int rb = 0; rb < RB; rb++) o[rb][dt] = mma<F16>(vf, pf[rb], o[rb][dt]);
     }
+  }
 }
 
 // Query fragments of rows row0 + 16 rb + r16 (row r of a kv head: its query r % G of sequence b0 + r / G)
@@ -423,12 +443,12 @@ __device__ __forceinline__ void own_part(const AttnArgs& A, const int* table, in
   }
   u32x4 qf[RB][D / 32];
   load_q<D, RB>(A, h, b0, row0, rows, r16, kg, qf);
-  float m[RB], l[RB];
-  f32x4 o[RB][D / 16];
+  float m[RB];
+  f32x4 l[RB], o[RB][D / 16];
 #pragma unroll
   for (int rb = 0; rb < RB; rb++) {
     m[rb] = -INFINITY;
-    l[rb] = 0.f;
+    l[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int dt = 0; dt < D / 16; dt++) o[rb][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -453,10 +473,9 @@ __device__ __forceinline__ void own_part(const AttnArgs& A, const int* table, in
   // D / 4 pieces of 16 bytes, swizzled with the row), then all add the four up
 #pragma unroll
   for (int rb = 0; rb < RB; rb++) {
-    l[rb] = groups_sum(l[rb]);
     if (kg == 0) {
       s_m[wv][16 * rb + r16] = m[rb];
-      s_l[wv][16 * rb + r16] = pages.bad ? NAN : l[rb];
+      s_l[wv][16 * rb + r16] = pages.bad ? NAN : l[rb][0];
     }
   }
   __syncthreads();
@@ -517,12 +536,12 @@ __device__ __forceinline__ void prefix_part(const AttnArgs& A, int h, int row0, 
   u32x4 qf[RB][D / 32];
   const int mine = row0 + 16 * RB * wv;
   load_q<D, RB>(A, h, 0, mine, rows, r16, kg, qf);
-  float m[RB], l[RB];
-  f32x4 o[RB][D / 16];
+  float m[RB];
+  f32x4 l[RB], o[RB][D / 16];
 #pragma unroll
   for (int rb = 0; rb < RB; rb++) {
     m[rb] = -INFINITY;
-    l[rb] = 0.f;
+    l[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int dt = 0; dt < D / 16; dt++) o[rb][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -538,7 +557,7 @@ __device__ __forceinline__ void prefix_part(const AttnArgs& A, int h, int row0, 
 #pragma unroll
   for (int rb = 0; rb < RB; rb++) {
     const int r = mine + 16 * rb + r16;
-    const float sum = bad ? NAN : groups_sum(l[rb]);
+    const float sum = bad ? NAN : l[rb][0];
     if (r < rows)
 #pragma unroll
       for (int dt = 0; dt < D / 16; dt++) store_o<F16, D>(A, slot, h, 0, r, 16 * dt + 4 * kg, o[rb][dt], m[rb], sum);
@@ -560,10 +579,14 @@ __global__ void __launch_bounds__(64 * AW, 2) attn_kernel(AttnArgs A) {
   __shared__ float s_m[AW][64], s_l[AW][64];
   static_assert(sizeof(s_kv) == AW * 2 * KS * D * 2, "the two forms take the same LDS");
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&s_kv[0];
-  int id = blockIdx.x;
+  // parts of the prefix and of own rows alternate, a workgroup a CU of each, while there are both
+  const int n_prefix = A.hkv * A.prefix_tiles * A.np, n_own = A.hkv * A.own_tiles * A.batch * A.ns;
+  const int runs = min(n_prefix, n_own) / NUM_CUS, bid = blockIdx.x, run = bid / NUM_CUS, rest = bid - runs * NUM_CUS;
+  const bool prefix = run < 2 * runs ? run % 2 == 0 : rest < n_prefix;
+  int id = run < 2 * runs ? run / 2 * NUM_CUS + bid % NUM_CUS : rest < n_prefix ? rest : bid - n_prefix;
   const int h = id % A.hkv;  // (fastest: with 8 kv heads each XCD reads one head's rows)
   id /= A.hkv;
-  if (id < A.prefix_tiles * A.np) {
+  if (prefix) {
     const int rows = A.batch * A.g, row0 = tile_rows(FORM) * (id % A.prefix_tiles), part = id / A.prefix_tiles;
     const int ch = part_keys(A.prefix_len, A.np), lo = part * ch, hi = min(A.prefix_len, lo + ch);
     if constexpr (FORM <= ROWS32)
@@ -572,7 +595,6 @@ __global__ void __launch_bounds__(64 * AW, 2) attn_kernel(AttnArgs A) {
       prefix_part<F16, D, FORM == ROWS64 ? 1 : 2>(A, h, row0, rows, lo, hi, part, lds);
     return;
   }
-  id -= A.prefix_tiles * A.np;
   const int tile = id % A.own_tiles;
   id /= A.own_tiles;
   const int b = id % A.batch, part = id / A.batch;
@@ -654,8 +676,9 @@ __global__ void __launch_bounds__(256) combine_kernel(AttnArgs A) {
 // of equals first; a score that is not a number counts as the greatest.
 //
 // One workgroup a (kv head, sequence): 16 lanes take a page (8 dims each at 128), the scores go to LDS
-// as unsigned 64-bit keys in the order of the scores, a radix selection by 8 bits finds the last key
-// that is chosen, and a scan writes the chosen pages in ascending order.
+// as unsigned 64-bit keys in the order of the scores. Up to 1024 of them are ranked by counting the
+// greater ones (one pass and one barrier); of more, a radix selection by 8 bits finds the last key that is
+// chosen. The chosen pages are written in ascending order.
 constexpr int ST = 1024;              // threads
 
 __device__ __forceinline__ uint64_t order_key(double x) {
@@ -677,7 +700,7 @@ __global__ void __launch_bounds__(ST) select_kernel(SelectArgs A) {
   const int* table = A.tables + (size_t)b * A.t_sb;
   int* chosen = A.chosen + ((size_t)b * A.hkv + h) * A.top;
   int* pages = A.pages + ((size_t)b * A.hkv + h) * A.top;
-  const int count = min(used, A.top);
+  const int count = min(used, A.top), n = used - 1;  // n: pages with a score
   if (h == 0 && tid == 0) A.sub_lens[b] = count == 0 ? 0 : ((count - 1) << A.lp) + ((len - 1) & ((1 << A.lp) - 1)) + 1;
   for (int i = count + tid; i < A.top; i += ST) chosen[i] = -1, pages[i] = -1;
   if (used <= A.top) {
@@ -699,31 +722,71 @@ __global__ void __launch_bounds__(ST) select_kernel(SelectArgs A) {
     double ql[8], qh[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) ql[i] = s_q[0][8 * c + i], qh[i] = s_q[1][8 * c + i];
-    for (int p = tid / LPP; p < used - 1; p += PPW) {
-      const int id = table[p];
-      double x = INFINITY;  // a page outside the pool is chosen: its sequence's outputs are then not numbers
-      if (id >= 0 && id < A.num_pages) {
-        const uint16_t* bd = A.bounds + ((size_t)id * A.hkv + h) * 2 * D + 8 * c;
-        float lo[8], hi[8];
-        to_f32x8<F16>(*(gu32x4*)bd, lo);
-        to_f32x8<F16>(*(gu32x4*)(bd + D), hi);
-        x = 0.0;
+    // (four pages at a time: their ids, then their bounds, are in flight together)
+    for (int p0 = tid / LPP; p0 < n; p0 += 4 * PPW) {
+      int id[4];
+      u32x4 lo[4], hi[4];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          x = fma((double)lo[i], ql[i], x);
-          x = fma((double)hi[i], qh[i], x);
-        }
+      for (int u = 0; u < 4; u++) id[u] = *(gint*)(table + min(p0 + PPW * u, n - 1));
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const int at = id[u] >= 0 && id[u] < A.num_pages ? id[u] : 0;
+        const uint16_t* bd = A.bounds + ((size_t)at * A.hkv + h) * 2 * D + 8 * c;
+        lo[u] = *(gu32x4*)bd;
+        hi[u] = *(gu32x4*)(bd + D);
       }
 #pragma unroll
-      for (int off = LPP / 2; off > 0; off >>= 1) x += __shfl_xor(x, off, LPP);
-      if (c == 0) s_key[p] = order_key(x);
+      for (int u = 0; u < 4; u++) {
+        float lf[8], hf[8];
+        to_f32x8<F16>(lo[u], lf);
+        to_f32x8<F16>(hi[u], hf);
+        double x = 0.0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          x = fma((double)lf[i], ql[i], x);
+          x = fma((double)hf[i], qh[i], x);
+        }
+#pragma unroll
+        for (int off = LPP / 2; off > 0; off >>= 1) x += __shfl_xor(x, off, LPP);
+        // (a page outside the pool is chosen: its sequence's outputs are then not numbers)
+        if (id[u] < 0 || id[u] >= A.num_pages) x = INFINITY;
+        if (c == 0 && p0 + PPW * u < n) s_key[p0 + PPW * u] = order_key(x);
+      }
     }
   }
+  __syncthreads();
+  const uint64_t below = (1ull << lane) - 1;
+  if (n <= ST) {
+    // ---- few keys: the rank of each, counted by `per` neighbouring lanes; those of a rank below top - 1 are chosen
+    int per = 1;
+    while (per < 64 && 2 * per * n <= ST) per *= 2;
+    const int i = tid / per;
+    uint32_t rank = 0;
+    if (i < n) {
+      const uint64_t k = s_key[i];
+      for (int j = tid % per; j < n; j += per) {
+        const uint64_t y = s_key[j];
+        rank += y > k || (y == k && j < i);
+      }
+    }
+    for (int off = 1; off < per; off *= 2) rank += __shfl_xor(rank, off, 64);
+    const bool take = i < n && tid % per == 0 && rank < (uint32_t)A.top - 1;
+    const uint64_t all = __ballot(take);
+    if (lane == 0) s_cnt[0][wv] = __popcll(all);
+    __syncthreads();
+    uint32_t at = __popcll(all & below);
+    for (int w = 0; w < wv; w++) at += s_cnt[0][w];
+    if (take) {
+      chosen[at] = i;
+      pages[at] = table[i];
+    }
+    if (tid == 0) chosen[A.top - 1] = n, pages[A.top - 1] = table[n];
+    return;
+  }
   // ---- the want-th greatest of used - 1 keys, 8 bits at a time from the top
-  const int n = used - 1;
   uint32_t want = A.top - 1;
   uint64_t prefix = 0, mask = 0;
-  if (want > 0)
+  if (want > 0) {
     for (int shift = 56; shift >= 0; shift -= 8) {
       if (tid < 256) s_hist[tid] = 0;
       __syncthreads();
@@ -757,15 +820,13 @@ __global__ void __launch_bounds__(ST) select_kernel(SelectArgs A) {
       mask |= 255ull << shift;
       want = s_sel[1];
     }
-  else
-    __syncthreads();
+  }
   // ---- keys above the last chosen one, and the first `want` of its equals, in ascending order
   uint32_t eq0 = 0, out0 = 0;
   for (int i0 = 0; i0 < n && A.top > 1; i0 += ST) {
     const int i = i0 + tid;
     const uint64_t k = i < n ? s_key[i] : 0;
     const bool gt = i < n && k > prefix, eq = i < n && k == prefix;
-    const uint64_t below = (1ull << lane) - 1;
     const uint64_t be = __ballot(eq), bg = __ballot(gt);
     if (lane == 0) s_cnt[0][wv] = __popcll(be), s_cnt[1][wv] = __popcll(bg);
     __syncthreads();
@@ -884,7 +945,11 @@ AttnPlan plan_attention(int batch, int hkv, int g, int d, int prefix_len, int ma
   };
   if (prefix_len > 0) {
     p.prefix_tiles = (rows + tile_rows(p.form) - 1) / tile_rows(p.form);
+#ifdef PWANT
+    p.np = parts(prefix_len, (long long)hkv * p.prefix_tiles * 512 / PWANT);
+#else
     p.np = parts(prefix_len, (long long)hkv * p.prefix_tiles);
+#endif
   }
   if (max_len > 0) p.ns = parts(max_len, (long long)batch * hkv * p.own_tiles);
   const size_t rows_all = p.np + p.ns == 1 ? 0 : (size_t)(p.np + p.ns) * batch * hkv * g;

@@ -18,6 +18,7 @@ no CPU fallback: tensors are on the GPU. Wrong types, shapes, strides or page id
 from __future__ import annotations
 
 import ctypes
+import functools
 import heapq
 import math
 
@@ -33,46 +34,49 @@ _DTYPES = {torch.bfloat16: _abi.MQ_BF16, torch.float16: _abi.MQ_FP16}
 
 def _call(name: str, device: torch.device, *args) -> None:
     """C ABI entry `name` with `args` and the current stream of `device`, on that device."""
-    _need(device.type == "cuda", f"expected tensors on the GPU, got {device}")
-    if device.index != torch.cuda.current_device():
+    if device.type != "cuda":
+        raise ValueError(f"expected tensors on the GPU, got {device}")
+    if device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
             return _call(name, device, *args)
-    _abi.check(getattr(_abi.lib(), name)(*args, torch.cuda.current_stream().cuda_stream), name)
-
-
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
+    status = getattr(_abi.lib(), name)(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    if status:
+        _abi.check(status, name)
 
 
 def _like(t, name: str, dtype, device, shape=None) -> None:
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or (shape is not None and tuple(t.shape) != shape):
-        raise ValueError(f"{name}: expected {dtype} {'' if shape is None else list(shape)} on {device}, got "
-                         f"{(t.dtype, list(t.shape), str(t.device)) if isinstance(t, torch.Tensor) else t}")
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or (shape is not None and t.shape != shape):
+        got = (t.dtype, list(t.shape), str(t.device)) if isinstance(t, torch.Tensor) else t
+        raise ValueError(f"{name}: expected {dtype} {'' if shape is None else list(shape)} on {device}, got {got}")
 
 
 def _pool(k_pages, v_pages, bounds, layered: bool) -> _abi.MqPagePool:
     """The pool's descriptor, after its checks. layered: [layers, ...], else one layer's [pages, ...]."""
     dims = 5 if layered else 4
-    _need(isinstance(k_pages, torch.Tensor) and k_pages.dim() == dims and k_pages.dtype in _DTYPES,
-          f"k_pages: expected a tensor of {dims} dimensions, bfloat16 or float16")
-    shape = tuple(k_pages.shape)
-    _like(v_pages, "v_pages", k_pages.dtype, k_pages.device, shape)
+    if not isinstance(k_pages, torch.Tensor) or k_pages.dim() != dims or k_pages.dtype not in _DTYPES:
+        raise ValueError(f"k_pages: expected a tensor of {dims} dimensions, bfloat16 or float16")
+    shape, dtype, device = k_pages.shape, k_pages.dtype, k_pages.device
+    _like(v_pages, "v_pages", dtype, device, shape)
     pages, heads, page, d = shape[-4:]
-    _need(page in PAGE_SIZES and d in HEAD_DIMS and pages > 0 and heads > 0 and shape[0] > 0,
-          f"k_pages: page size {page} (of {PAGE_SIZES}) or head dim {d} (of {HEAD_DIMS}) or a size of zero")
-    _need(k_pages.is_contiguous() and v_pages.is_contiguous(), "k_pages, v_pages: expected contiguous tensors")
+    if page not in PAGE_SIZES or d not in HEAD_DIMS or pages == 0 or heads == 0 or shape[0] == 0:
+        raise ValueError(f"k_pages: page size {page} (of {PAGE_SIZES}) or head dim {d} (of {HEAD_DIMS}) or a size of zero")
+    if not k_pages.is_contiguous() or not v_pages.is_contiguous():
+        raise ValueError("k_pages, v_pages: expected contiguous tensors")
+    at = None
     if bounds is not None:
-        _like(bounds, "bounds", k_pages.dtype, k_pages.device, shape[:-2] + (2, d))
-        _need(bounds.is_contiguous(), "bounds: expected a contiguous tensor")
-    return _abi.MqPagePool(k_pages.data_ptr(), v_pages.data_ptr(), None if bounds is None else bounds.data_ptr(),
-                           shape[0] if layered else 1, pages, heads, page, d, _DTYPES[k_pages.dtype])
+        _like(bounds, "bounds", dtype, device, shape[:-2] + (2, d))
+        if not bounds.is_contiguous():
+            raise ValueError("bounds: expected a contiguous tensor")
+        at = bounds.data_ptr()
+    return _abi.MqPagePool(k_pages.data_ptr(), v_pages.data_ptr(), at, shape[0] if layered else 1, pages, heads, page, d,
+                           _DTYPES[dtype])
 
 
 def _page_list(ids, name: str, num_pages: int):
-    """A host list of page ids as a C array."""
+    """A host list of page ids, and as a C array."""
     ids = [int(i) for i in ids]
-    _need(all(0 <= i < num_pages for i in ids), f"{name}: page ids must be in [0, {num_pages})")
+    if ids and (min(ids) < 0 or max(ids) >= num_pages):
+        raise ValueError(f"{name}: page ids must be in [0, {num_pages})")
     return ids, (ctypes.c_int * len(ids))(*ids)
 
 
@@ -82,8 +86,10 @@ def copy_pages(k_pages, v_pages, src, dst, bounds=None) -> None:
     pool = _pool(k_pages, v_pages, bounds, True)
     src, c_src = _page_list(src, "src", pool.num_pages)
     dst, c_dst = _page_list(dst, "dst", pool.num_pages)
-    _need(len(src) == len(dst), "src and dst: expected lists of one length")
-    _need(len(set(dst)) == len(dst) and not set(dst) & set(src), "dst: a page twice, or one that is copied from as well")
+    if not (len(src) == len(dst)):
+        raise ValueError("src and dst: expected lists of one length")
+    if not (len(set(dst)) == len(dst) and not set(dst) & set(src)):
+        raise ValueError("dst: a page twice, or one that is copied from as well")
     if src:
         _call("mq_pages_copy", k_pages.device, pool, c_src, c_dst, len(src))
 
@@ -92,15 +98,19 @@ def _move(name, k_cache, v_cache, k_pages, v_pages, pages, length, bounds) -> No
     pool = _pool(k_pages, v_pages, bounds, True)
     pages, c_pages = _page_list(pages, "pages", pool.num_pages)
     length = int(length)
-    _need(length >= 0 and len(pages) == -(-length // pool.page_size),
-          f"pages: {length} rows need {-(-length // pool.page_size)} pages of {pool.page_size}, got {len(pages)}")
-    _need(len(set(pages)) == len(pages), "pages: a page twice")
-    _need(isinstance(k_cache, torch.Tensor) and k_cache.dim() == 4, "k_cache: expected [layers, kv heads, positions, head dim]")
+    if not (length >= 0 and len(pages) == -(-length // pool.page_size)):
+        raise ValueError(f"pages: {length} rows need {-(-length // pool.page_size)} pages of {pool.page_size}, got {len(pages)}")
+    if len(set(pages)) != len(pages):
+        raise ValueError("pages: a page twice")
+    if not (isinstance(k_cache, torch.Tensor) and k_cache.dim() == 4):
+        raise ValueError("k_cache: expected [layers, kv heads, positions, head dim]")
     shape = (pool.num_layers, pool.num_kv_heads, k_cache.shape[2], pool.head_dim)
     for t, what in ((k_cache, "k_cache"), (v_cache, "v_cache")):
         _like(t, what, k_pages.dtype, k_pages.device, shape)
-        _need(t.is_contiguous(), f"{what}: expected a contiguous tensor")
-    _need(length <= shape[2], f"length {length} exceeds the cache's {shape[2]} positions")
+        if not t.is_contiguous():
+            raise ValueError(f"{what}: expected a contiguous tensor")
+    if length > shape[2]:
+        raise ValueError(f"length {length} exceeds the cache's {shape[2]} positions")
     if length:
         _call(name, k_pages.device, pool, c_pages, length, k_cache.data_ptr(), v_cache.data_ptr(), shape[2])
 
@@ -124,21 +134,21 @@ def _rows(t, name: str, like, shape) -> tuple[int, int]:
     sb, sh, sd = t.stride()
     # (a stride over one element is never used, whatever it says)
     sb, sh = (sb if shape[0] > 1 else 0), (sh if shape[1] > 1 else 0)
-    _need(sd == 1 and sb >= 0 and sh >= 0 and sb % 8 == 0 and sh % 8 == 0 and t.data_ptr() % 16 == 0,
-          f"{name}: expected rows of contiguous elements that begin at multiples of 16 bytes, got strides {t.stride()}")
+    if not (sd == 1 and sb >= 0 and sh >= 0 and sb % 8 == 0 and sh % 8 == 0 and t.data_ptr() % 16 == 0):
+        raise ValueError(f"{name}: expected rows of contiguous elements that begin at multiples of 16 bytes, got strides {t.stride()}")
     return sb, sh
 
 
 def _tables(tables, lens, batch: int, device) -> tuple[int, int]:
     """(row stride, width) of int32 page tables [batch, width]."""
-    _need(isinstance(tables, torch.Tensor) and tables.dim() == 2 and tables.shape[0] == batch
-          and 1 <= tables.shape[1] <= _abi.MQ_MAX_TABLE_WIDTH,
-          f"tables: expected int32 [{batch}, 1 .. {_abi.MQ_MAX_TABLE_WIDTH}]")
+    if not (isinstance(tables, torch.Tensor) and tables.dim() == 2 and tables.shape[0] == batch
+            and 1 <= tables.shape[1] <= _abi.MQ_MAX_TABLE_WIDTH):
+        raise ValueError(f"tables: expected int32 [{batch}, 1 .. {_abi.MQ_MAX_TABLE_WIDTH}]")
     _like(tables, "tables", torch.int32, device)
     _like(lens, "lens", torch.int32, device, (batch,))
     width = tables.shape[1]
-    _need((width == 1 or tables.stride(1) == 1) and (batch == 1 or lens.stride(0) == 1) and tables.stride(0) >= 0,
-          "tables, lens: expected contiguous rows")
+    if not ((width == 1 or tables.stride(1) == 1) and (batch == 1 or lens.stride(0) == 1) and tables.stride(0) >= 0):
+        raise ValueError("tables, lens: expected contiguous rows")
     return (tables.stride(0) if batch > 1 else 0), width
 
 
@@ -148,7 +158,8 @@ def append_rows(k, v, k_pages, v_pages, tables, lens, bounds=None) -> None:
     with `bounds` the page's bounds. `lens` itself does not change. No two sequences may append to
     one page; a row for a position behind its table, or for a page outside the pool, is dropped."""
     pool = _pool(k_pages, v_pages, bounds, False)
-    _need(isinstance(k, torch.Tensor) and k.dim() == 3 and 1 <= k.shape[0] <= 65535, "k: expected [batch, kv heads, head dim]")
+    if not (isinstance(k, torch.Tensor) and k.dim() == 3 and 1 <= k.shape[0] <= 65535):
+        raise ValueError("k: expected [batch, kv heads, head dim]")
     shape = (k.shape[0], pool.num_kv_heads, pool.head_dim)
     k_sb, k_sh = _rows(k, "k", k_pages, shape)
     v_sb, v_sh = _rows(v, "v", k_pages, shape)
@@ -158,28 +169,31 @@ def append_rows(k, v, k_pages, v_pages, tables, lens, bounds=None) -> None:
 
 
 def _query(q, out, pool, like) -> tuple[torch.Tensor, tuple[int, int], tuple[int, int]]:
-    _need(isinstance(q, torch.Tensor) and q.dim() == 3 and 1 <= q.shape[0] <= 65535 and q.shape[1] > 0
-          and q.shape[1] % pool.num_kv_heads == 0,
-          f"q: expected [batch, a multiple of {pool.num_kv_heads} heads, {pool.head_dim}]")
+    if not (isinstance(q, torch.Tensor) and q.dim() == 3 and 1 <= q.shape[0] <= 65535 and 0 < q.shape[1] <= 16384
+            and q.shape[1] % pool.num_kv_heads == 0):
+        raise ValueError(f"q: expected [batch, a multiple of {pool.num_kv_heads} heads, {pool.head_dim}]")
     shape = (q.shape[0], q.shape[1], pool.head_dim)
     strides = _rows(q, "q", like, shape)
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        return torch.empty(shape, dtype=q.dtype, device=q.device), strides, (shape[1] * shape[2], shape[2])
     out_strides = _rows(out, "out", like, shape)
-    _need((shape[0] == 1 or out_strides[0] > 0) and (shape[1] == 1 or out_strides[1] > 0), "out: rows that overlap")
+    if (shape[0] > 1 and out_strides[0] == 0) or (shape[1] > 1 and out_strides[1] == 0):
+        raise ValueError("out: rows that overlap")
     return out, strides, out_strides
 
 
 def _scale(scale, head_dim: int) -> float:
     scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
-    _need(scale > 0 and math.isfinite(scale), "scale must be positive and finite")
+    if not (scale > 0 and math.isfinite(scale)):
+        raise ValueError("scale must be positive and finite")
     return scale
 
 
-def _workspace(pool, heads, batch, prefix_len, max_len, top, device) -> torch.Tensor:
-    n = ctypes.c_size_t()
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(kv_heads: int, head_dim: int, heads: int, batch: int, prefix_len: int, max_len: int, top: int) -> int:
+    n, pool = ctypes.c_size_t(), _abi.MqPagePool(num_kv_heads=kv_heads, head_dim=head_dim)
     _abi.check(_abi.lib().mq_attention_workspace(pool, heads, batch, prefix_len, max_len, top, n), "mq_attention_workspace")
-    return torch.empty(max(n.value, 16), dtype=torch.uint8, device=device)
+    return max(n.value, 16)
 
 
 def shared_prefix_attention(q, k_pages, v_pages, prefix_pages, prefix_len: int, tables, lens, scale: float | None = None,
@@ -187,7 +201,7 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix_pages, prefix_len: int, 
     """Attention of one query token a sequence, `q` `[batch, query heads, head dim]`, over a prefix that all
     sequences share and the sequence's own rows behind it: softmax(scale q K^T) V with K, V = prefix
     rows 0 .. prefix_len - 1, then own rows 0 .. lens[b] - 1. The prefix is read once for all sequences
-    (for each 64 query rows of a kv head).
+    (for each 128 query rows of a kv head).
 
     One layer's pool; `prefix_pages` int32 on the GPU, `prefix_len` a host number (0: no prefix);
     `tables` int32 `[batch, width]` (rows may be a slice of wider ones), `lens` int32 `[batch]`. A sequence
@@ -199,18 +213,22 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix_pages, prefix_len: int, 
     batch, heads = q.shape[0], q.shape[1]
     t_sb, width = _tables(tables, lens, batch, k_pages.device)
     prefix_len = int(prefix_len)
-    _need(prefix_len >= 0, "prefix_len must not be negative")
+    if prefix_len < 0:
+        raise ValueError("prefix_len must not be negative")
     if prefix_len:
         _like(prefix_pages, "prefix_pages", torch.int32, k_pages.device)
-        _need(prefix_pages.dim() == 1 and prefix_pages.is_contiguous() and prefix_pages.numel() >= -(-prefix_len // pool.page_size),
-              f"prefix_pages: expected at least {-(-prefix_len // pool.page_size)} contiguous page ids")
+        if not (prefix_pages.dim() == 1 and prefix_pages.is_contiguous()
+                and prefix_pages.numel() >= -(-prefix_len // pool.page_size)):
+            raise ValueError(f"prefix_pages: expected at least {-(-prefix_len // pool.page_size)} contiguous page ids")
     whole = width * pool.page_size
     max_len = whole if max_len is None else min(int(max_len), whole)
-    _need(max_len > 0, "max_len must be positive")
-    ws = _workspace(pool, heads, batch, prefix_len, max_len, 0, q.device)
+    if max_len < 1:
+        raise ValueError("max_len must be positive")
+    ws_bytes = _workspace_bytes(pool.num_kv_heads, pool.head_dim, heads, batch, prefix_len, max_len, 0)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
     _call("mq_shared_prefix_attention", k_pages.device, pool, q.data_ptr(), q_sb, q_sh, out.data_ptr(), o_sb, o_sh, heads, batch,
           prefix_pages.data_ptr() if prefix_len else None, prefix_len, tables.data_ptr(), t_sb, width, lens.data_ptr(), max_len,
-          _scale(scale, pool.head_dim), ws.data_ptr(), ws.numel())
+          _scale(scale, pool.head_dim), ws.data_ptr(), ws_bytes)
     return out
 
 
@@ -224,14 +242,17 @@ def sparse_attention(q, k_pages, v_pages, bounds, tables, lens, top_pages: int, 
 
     Returns (out, chosen): `chosen` int32 `[batch, kv heads, top_pages]`, the pages' numbers in the
     sequence's table, ascending, then -1. The rest as `shared_prefix_attention` without a prefix."""
-    _need(bounds is not None, "bounds: expected a tensor")
+    if bounds is None:
+        raise ValueError("bounds: expected a tensor")
     pool = _pool(k_pages, v_pages, bounds, False)
     out, (q_sb, q_sh), (o_sb, o_sh) = _query(q, out, pool, k_pages)
     batch, heads, top = q.shape[0], q.shape[1], int(top_pages)
     t_sb, width = _tables(tables, lens, batch, k_pages.device)
-    _need(1 <= top <= _abi.MQ_MAX_TABLE_WIDTH, f"top_pages must be in [1, {_abi.MQ_MAX_TABLE_WIDTH}]")
+    if not 1 <= top <= _abi.MQ_MAX_TABLE_WIDTH:
+        raise ValueError(f"top_pages must be in [1, {_abi.MQ_MAX_TABLE_WIDTH}]")
     chosen = torch.empty(batch, pool.num_kv_heads, top, dtype=torch.int32, device=q.device)
-    ws = _workspace(pool, heads, batch, 0, min(top, width) * pool.page_size, top, q.device)
+    ws_bytes = _workspace_bytes(pool.num_kv_heads, pool.head_dim, heads, batch, 0, min(top, width) * pool.page_size, top)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
     _call("mq_sparse_attention", k_pages.device, pool, q.data_ptr(), q_sb, q_sh, out.data_ptr(), o_sb, o_sh, chosen.data_ptr(), heads,
-          batch, tables.data_ptr(), t_sb, width, lens.data_ptr(), top, _scale(scale, pool.head_dim), ws.data_ptr(), ws.numel())
+          batch, tables.data_ptr(), t_sb, width, lens.data_ptr(), top, _scale(scale, pool.head_dim), ws.data_ptr(), ws_bytes)
     return out, chosen
