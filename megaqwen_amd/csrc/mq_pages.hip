@@ -676,15 +676,65 @@ __global__ void __launch_bounds__(256) combine_kernel(AttnArgs A) {
 // of equals first; a score that is not a number counts as the greatest.
 //
 // One workgroup a (kv head, sequence): 16 lanes take a page (8 dims each at 128), the scores go to LDS
-// as unsigned 64-bit keys in the order of the scores. Up to 1024 of them are ranked by counting the
-// greater ones (one pass and one barrier); of more, a radix selection by 8 bits finds the last key that is
-// chosen. The chosen pages are written in ascending order.
+// as unsigned 64-bit keys in the order of the scores. Of up to 1024 of them one wave finds the last that is
+// chosen, of more the workgroup, by a radix selection 8 bits at a time. The chosen pages are written in
+// ascending order.
 constexpr int ST = 1024;              // threads
 
 __device__ __forceinline__ uint64_t order_key(double x) {
   const uint64_t u = __builtin_bit_cast(uint64_t, x + 0.0);  // (-0 counts as 0)
   if (x != x) return ~0ull;
   return u >> 63 ? ~u : u | 1ull << 63;
+}
+
+// (the lane orders of row16_sum)
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xF, 0xF, true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, true);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// Of n <= 64 R keys, one wave: the `want` greatest, the lower of equals first, in ascending order. The least
+// chosen key is built from the top bit down, each bit by counting the keys that are at least as great,
+// until the count fits (some 20 bits for scores that differ) or the key is complete.
+template <int R>
+__device__ __forceinline__ void choose(const uint64_t* key, const int* id, int n, int want, int* chosen, int* pages, int lane) {
+  if (want == 0) return;
+  uint64_t k[R], least = 0;
+#pragma unroll
+  for (int r = 0; r < R; r++) k[r] = 64 * r + lane < n ? key[64 * r + lane] : 0;  // (a key is never 0)
+  bool fits = false;
+  for (int bit = 63; bit >= 0 && !fits; bit--) {
+    const uint64_t x = least | 1ull << bit;
+    int count = 0;
+#pragma unroll
+    for (int r = 0; r < R; r++) count += (int)__popcll(__ballot(k[r] >= x));
+    if (count >= want) least = x;
+    fits = count == want;
+  }
+  int equals = 0;  // keys equal to `least` that are chosen
+  if (!fits) {
+    equals = want;
+#pragma unroll
+    for (int r = 0; r < R; r++) equals -= (int)__popcll(__ballot(k[r] > least));
+  }
+  const uint64_t below = (1ull << lane) - 1;
+  int at = 0;
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    const uint64_t eq = __ballot(k[r] == least);
+    const bool take = k[r] > least || (k[r] == least && (fits || (int)__popcll(eq & below) < equals));
+    const uint64_t all = __ballot(take);
+    if (take) {
+      const int to = at + (int)__popcll(all & below);
+      chosen[to] = 64 * r + lane;
+      pages[to] = id[64 * r + lane];
+    }
+    at += (int)__popcll(all);
+    equals = max(0, equals - (int)__popcll(eq));
+  }
 }
 
 template <bool F16, int D>
@@ -695,6 +745,7 @@ __global__ void __launch_bounds__(ST) select_kernel(SelectArgs A) {
   __shared__ uint32_t s_hist[256];
   __shared__ uint32_t s_sel[2];    // the digit chosen, keys still wanted in it
   __shared__ uint32_t s_cnt[2][ST / 64];
+  __shared__ int s_id[ST];  // (of up to ST pages)
   const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const int len = max(0, min(A.lens[b] + A.len_add, A.width << A.lp)), used = (len + (1 << A.lp) - 1) >> A.lp;
   const int* table = A.tables + (size_t)b * A.t_sb;
@@ -707,6 +758,11 @@ __global__ void __launch_bounds__(ST) select_kernel(SelectArgs A) {
     for (int i = tid; i < used; i += ST) chosen[i] = i, pages[i] = table[i];
     return;
   }
+  // (the first ids are asked for before the queries, whose sums need a barrier)
+  int id[4];
+#pragma unroll
+  for (int u = 0; u < 4; u++) id[u] = *(gint*)(table + min(tid / LPP + PPW * u, n - 1));
+  const int last = *(gint*)(table + n);
   if (tid < D) {
     double pos = 0.0, neg = 0.0;
     for (int g = 0; g < A.g; g++) {
@@ -722,12 +778,12 @@ __global__ void __launch_bounds__(ST) select_kernel(SelectArgs A) {
     double ql[8], qh[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) ql[i] = s_q[0][8 * c + i], qh[i] = s_q[1][8 * c + i];
-    // (four pages at a time: their ids, then their bounds, are in flight together)
+    // four pages at a time: their ids, then their bounds, are in flight together
     for (int p0 = tid / LPP; p0 < n; p0 += 4 * PPW) {
-      int id[4];
-      u32x4 lo[4], hi[4];
+      if (p0 >= 4 * PPW)
 #pragma unroll
-      for (int u = 0; u < 4; u++) id[u] = *(gint*)(table + min(p0 + PPW * u, n - 1));
+        for (int u = 0; u < 4; u++) id[u] = *(gint*)(table + min(p0 + PPW * u, n - 1));
+      u32x4 lo[4], hi[4];
 #pragma unroll
       for (int u = 0; u < 4; u++) {
         const int at = id[u] >= 0 && id[u] < A.num_pages ? id[u] : 0;
@@ -746,41 +802,28 @@ __global__ void __launch_bounds__(ST) select_kernel(SelectArgs A) {
           x = fma((double)lf[i], ql[i], x);
           x = fma((double)hf[i], qh[i], x);
         }
-#pragma unroll
-        for (int off = LPP / 2; off > 0; off >>= 1) x += __shfl_xor(x, off, LPP);
+        x += dpp64<0xB1>(x);
+        x += dpp64<0x4E>(x);
+        x += dpp64<0x141>(x);
+        if (LPP == 16) x += dpp64<0x140>(x);
         // (a page outside the pool is chosen: its sequence's outputs are then not numbers)
         if (id[u] < 0 || id[u] >= A.num_pages) x = INFINITY;
-        if (c == 0 && p0 + PPW * u < n) s_key[p0 + PPW * u] = order_key(x);
+        if (c == 0 && p0 + PPW * u < n) {
+          s_key[p0 + PPW * u] = order_key(x);
+          if (n <= ST) s_id[p0 + PPW * u] = id[u];
+        }
       }
     }
   }
   __syncthreads();
   const uint64_t below = (1ull << lane) - 1;
   if (n <= ST) {
-    // ---- few keys: the rank of each, counted by `per` neighbouring lanes; those of a rank below top - 1 are chosen
-    int per = 1;
-    while (per < 64 && 2 * per * n <= ST) per *= 2;
-    const int i = tid / per;
-    uint32_t rank = 0;
-    if (i < n) {
-      const uint64_t k = s_key[i];
-      for (int j = tid % per; j < n; j += per) {
-        const uint64_t y = s_key[j];
-        rank += y > k || (y == k && j < i);
-      }
-    }
-    for (int off = 1; off < per; off *= 2) rank += __shfl_xor(rank, off, 64);
-    const bool take = i < n && tid % per == 0 && rank < (uint32_t)A.top - 1;
-    const uint64_t all = __ballot(take);
-    if (lane == 0) s_cnt[0][wv] = __popcll(all);
-    __syncthreads();
-    uint32_t at = __popcll(all & below);
-    for (int w = 0; w < wv; w++) at += s_cnt[0][w];
-    if (take) {
-      chosen[at] = i;
-      pages[at] = table[i];
-    }
-    if (tid == 0) chosen[A.top - 1] = n, pages[A.top - 1] = table[n];
+    if (wv > 0) return;
+    if (n <= 256)
+      choose<4>(s_key, s_id, n, A.top - 1, chosen, pages, lane);
+    else
+      choose<ST / 64>(s_key, s_id, n, A.top - 1, chosen, pages, lane);
+    if (lane == 0) chosen[A.top - 1] = n, pages[A.top - 1] = last;
     return;
   }
   // ---- the want-th greatest of used - 1 keys, 8 bits at a time from the top
@@ -848,7 +891,7 @@ __global__ void __launch_bounds__(ST) select_kernel(SelectArgs A) {
     eq0 += all_e;
     __syncthreads();
   }
-  if (tid == 0) chosen[A.top - 1] = n, pages[A.top - 1] = table[n];
+  if (tid == 0) chosen[A.top - 1] = n, pages[A.top - 1] = last;
 }
 
 // ------------------------------------------------------------------ launches
