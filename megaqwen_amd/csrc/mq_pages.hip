@@ -234,12 +234,18 @@ typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s lds_v4s;
 typedef const __attribute__((address_space(3))) u32x4 lds_u32x4;
 typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
+typedef __attribute__((address_space(3))) uint8_t lds_byte;
 typedef const __attribute__((address_space(1))) int gint;
 
 // the swizzle of a row's 16-byte pieces (D / 8 of them): 256-byte rows all start at the same bank,
 // 128-byte ones in pairs
 template <int D>
 __device__ __forceinline__ int swz(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
+
+// A value that a plain load brought, used here: the compiler, which does not count the DMA instructions, waits
+// for it at this place, and not (for every load and DMA under way) at its next use inside a loop
+template <class T>
+__device__ __forceinline__ void settled(T& x) { asm volatile("" : "+v"(x)); }
 
 // The page ids of a run of keys, 64 at a time, one a lane; asked for in ascending order.
 struct Pages {
@@ -249,11 +255,13 @@ struct Pages {
   __device__ __forceinline__ Pages(const int* t, int n, int page_lo, int page_last, int lane)
       : table(t), first(page_lo), last(page_last), num_pages(n), bad(false) {
     ids = *(gint*)(table + min(first + lane, last));
+    settled(ids);
   }
   __device__ __forceinline__ int operator()(int page, int lane) {
     if (page - first >= 64) {
       first = page;
       ids = *(gint*)(table + min(first + lane, last));
+      settled(ids);
     }
     const int id = __builtin_amdgcn_readlane(ids, page - first);
     if (id >= 0 && id < num_pages) return id;
@@ -265,14 +273,15 @@ struct Pages {
 // 16 consecutive keys from k0 (a multiple of 16, so of one page) of K or V, to LDS: NI DMA
 // instructions. Rows past k_last repeat it, from its page `clamp` (their scores are masked, and a
 // row that is not there is never read).
-template <int D>
+template <int D, bool ONCE>
 __device__ __forceinline__ void fetch16(const uint16_t* pool, size_t base, int k0, int k_last, int pmask, uint32_t dst, int lane) {
   constexpr int CPR = D / 8, RPI = 64 / CPR, NI = 16 / RPI;  // pieces a row, rows an instruction
 #pragma unroll
   for (int i = 0; i < NI; i++) {
     const int row = RPI * i + lane / CPR, key = min(k0 + row, k_last);
-    dma16(pool + base + (size_t)((key & pmask) * D + 8 * ((lane % CPR) ^ swz<D>(row))),
-          __builtin_amdgcn_readfirstlane(dst + 1024u * i));
+    const uint16_t* src = pool + base + (size_t)((key & pmask) * D + 8 * ((lane % CPR) ^ swz<D>(row)));
+    const uint32_t to = __builtin_amdgcn_readfirstlane(dst + 1024u * i);
+    if (ONCE) dma16_nt(src, to); else dma16(src, to);
   }
 }
 
@@ -304,17 +313,27 @@ __device__ __forceinline__ void attend_step(uint32_t kb, uint32_t vb, int left, 
                                             const u32x4 (&qf)[RB][D / 32], float (&m)[RB], f32x4 (&l)[RB],
                                             f32x4 (&o)[RB][D / 16], BeforeV before_v) {
   f32x4 sc[RB][NT];
+  // two key tiles at a time (2 RB chains of products that do not wait for each other); a pair's K fragments are
+  // read each as soon as its registers are free, beside the products of the pair before
+  u32x4 kf[2][D / 32];
+  auto load_k = [&](int t, int ks) {
+    kf[t & 1][ks] = *(lds_u32x4*)((const lds_byte*)(uintptr_t)(kb + (ka ^ (64u * ks))) + 32 * D * t);
+  };
 #pragma unroll
-  for (int t = 0; t < NT; t++) {
-    u32x4 kf[D / 32];
+  for (int ks = 0; ks < D / 32; ks++) load_k(0, ks), load_k(1, ks);
 #pragma unroll
-    for (int ks = 0; ks < D / 32; ks++) kf[ks] = *(lds_u32x4*)(uintptr_t)(kb + ((ka ^ (64u * ks)) + 32u * D * t));
+  for (int t = 0; t < NT; t += 2) {
 #pragma unroll
-    for (int rb = 0; rb < RB; rb++) {
-      f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int rb = 0; rb < RB; rb++) sc[rb][t] = sc[rb][t + 1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int ks = 0; ks < D / 32; ks++) a = mma<F16>(kf[ks], qf[rb][ks], a);
-      sc[rb][t] = a;
+    for (int ks = 0; ks < D / 32; ks++) {
+#pragma unroll
+      for (int rb = 0; rb < RB; rb++) {
+        sc[rb][t] = mma<F16>(kf[0][ks], qf[rb][ks], sc[rb][t]);
+        sc[rb][t + 1] = mma<F16>(kf[1][ks], qf[rb][ks], sc[rb][t + 1]);
+      }
+      if (t + 2 < NT) load_k(t + 2, ks), load_k(t + 3, ks);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
   if (left < 16 * NT) {
@@ -354,7 +373,18 @@ __device__ __forceinline__ void attend_step(uint32_t kb, uint32_t vb, int left, 
   before_v();
   constexpr uint32_t ONE = F16 ? 0x3c003c00u : 0x3f803f80u;
   const u32x4 ones = u32x4{ONE, ONE, ONE, ONE};
-  // (straight-line from here: the exponentials of one 32-key half run beside the products of the other)
+  // straight-line from here: the V fragments of a 32-key half are read before its exponentials, those of the
+  // next one each as soon as its registers are free, beside the products of this one
+  u32x4 vf[D / 16];
+  auto load_v = [&](int j, int dt) {
+    lds_byte* at = (lds_byte*)(uintptr_t)(vb + (va ^ (32u * dt))) + 64 * D * j;
+    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)at));
+    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 32 * D)));
+    vf[dt] = u32x4{lo.x, lo.y, hi.x, hi.y};
+  };
+#pragma unroll
+  for (int dt = 0; dt < D / 16; dt++) load_v(0, dt);
+  __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int j = 0; j < NT / 2; j++) {
     u32x4 pf[RB];
@@ -374,12 +404,12 @@ __device__ __forceinline__ void attend_step(uint32_t kb, uint32_t vb, int left, 
     for (int rb = 0; rb < RB; rb++) l[rb] = mma<F16>(ones, pf[rb], l[rb]);
 #pragma unroll
     for (int dt = 0; dt < D / 16; dt++) {
-      const uint32_t a = vb + (va ^ (32u * dt)) + 64u * D * j;
-      const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(uintptr_t)a));
-      const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(uintptr_t)(a + 32u * D)));
-      const u32x4 vf = u32x4{lo.x, lo.y, hi.x, hi.y};
 #pragma unroll
-      for (int rb = 0; rb < RB; rb++) o[rb][dt] = mma<F16>(vf, pf[rb], o[rb][dt]);
+      for (int rb = 0; rb < RB; rb++) o[rb][dt] = mma<F16>(vf[dt], pf[rb], o[rb][dt]);
+      if (j + 1 < NT / 2) {
+        load_v(j + 1, dt);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
   }
 }
@@ -395,6 +425,10 @@ __device__ __forceinline__ void load_q(const AttnArgs& A, int h, int b0, int row
 #pragma unroll
     for (int ks = 0; ks < D / 32; ks++) qf[rb][ks] = *(gu32x4*)(q + 32 * ks + 8 * kg);
   }
+#pragma unroll
+  for (int rb = 0; rb < RB; rb++)
+#pragma unroll
+    for (int ks = 0; ks < D / 32; ks++) settled(qf[rb][ks]);
 }
 
 // Where row r's result goes: part `slot` of the partial results, or, as the only part, the output.
@@ -432,8 +466,8 @@ __device__ __forceinline__ void own_part(const AttnArgs& A, const int* table, in
     base[1] = A.lp == 4 && k0 + 16 < k_hi ? (size_t)pages((k0 >> 4) + 1, lane) * page_elems + head_elems : base[0];
   };
   auto fetch = [&](const uint16_t* pool, int k0, uint32_t dst) {
-    fetch16<D>(pool, base[0], k0, k_hi - 1, pmask, dst, lane);
-    fetch16<D>(pool, base[1], k0 + 16, k_hi - 1, pmask, dst + HALF / 2, lane);
+    fetch16<D, true>(pool, base[0], k0, k_hi - 1, pmask, dst, lane);
+    fetch16<D, true>(pool, base[1], k0 + 16, k_hi - 1, pmask, dst + HALF / 2, lane);
   };
   int k0 = k_lo + KS * wv;
   if (k0 < k_hi) {
@@ -529,8 +563,8 @@ __device__ __forceinline__ void prefix_part(const AttnArgs& A, int h, int row0, 
   auto fetch = [&](int k0, uint32_t dst) {
     const int k = min(k0 + 16 * wv, k_hi - 1);
     const size_t base = (size_t)pages(k >> A.lp, lane) * page_elems + head_elems;
-    fetch16<D>(A.k, base, k0 + 16 * wv, k_hi - 1, pmask, dst + HALF / 4 * wv, lane);
-    fetch16<D>(A.v, base, k0 + 16 * wv, k_hi - 1, pmask, dst + HALF + HALF / 4 * wv, lane);
+    fetch16<D, false>(A.k, base, k0 + 16 * wv, k_hi - 1, pmask, dst + HALF / 4 * wv, lane);
+    fetch16<D, false>(A.v, base, k0 + 16 * wv, k_hi - 1, pmask, dst + HALF + HALF / 4 * wv, lane);
   };
   fetch(k_lo, lds);
   u32x4 qf[RB][D / 32];
@@ -972,29 +1006,31 @@ int append_rows(const AppendArgs& A, bool f16, hipStream_t stream) {
 // How an attention call is split. Query rows of the prefix go in tiles of up to 128, so that its keys are read
 // as few times as there are tiles; a sequence's own rows are shared by its G query heads a kv head only, in
 // tiles of 16. Keys are split until the launch has about two workgroups a CU, in parts of at least 128 keys.
+// Beside own rows the prefix takes fewer workgroups, so that it ends about when they do: each part's result
+// is another 4 D + 8 bytes a query row written and read (64 sequences behind 8192 shared rows with up to 512 own
+// ones 42.0 us with 512 workgroups for the prefix, 34.4 with 256, 29.6 with 128; 256 behind 15001 with up to
+// 1024 144, 127, 127; without own rows 52.6, 57.5, 90.9 for 16384). Its time is taken as 1.45 us for 64 keys
+// of a tile, one workgroup a CU, the own rows' as their bytes, half of the longest a sequence, at 5.4 TB/s.
 AttnPlan plan_attention(int batch, int hkv, int g, int d, int prefix_len, int max_len) {
   AttnPlan p{};
   constexpr int WANT = 512;
   const int rows = batch * g;
   p.form = rows <= 16 ? ROWS16 : rows <= 32 ? ROWS32 : rows <= 64 ? ROWS64 : ROWS128;
   p.own_tiles = (g + 15) / 16;
-  auto parts = [&](int len, long long tiles) {
+  auto parts = [&](int len, long long tiles, double want) {
     const int most = (len + UNIT - 1) / UNIT;
-    long long n = (WANT + tiles - 1) / tiles;
-    if (n > most) n = most;
-    if (n > MAX_PARTS / 2) n = MAX_PARTS / 2;
+    double n = ceil(want / (double)tiles);
+    n = fmax(1., fmin(n, fmin(most, MAX_PARTS / 2)));
     const int ch = part_keys(len, (int)n);
     return (len + ch - 1) / ch;  // (as many as have a key)
   };
   if (prefix_len > 0) {
     p.prefix_tiles = (rows + tile_rows(p.form) - 1) / tile_rows(p.form);
-#ifdef PWANT
-    p.np = parts(prefix_len, (long long)hkv * p.prefix_tiles * 512 / PWANT);
-#else
-    p.np = parts(prefix_len, (long long)hkv * p.prefix_tiles);
-#endif
+    const double tiles = (double)hkv * p.prefix_tiles;
+    const double us = tiles * ((prefix_len + TS - 1) / TS) * 1.45, own_us = (double)batch * hkv * max_len * d * 2 / 5.4e6;
+    p.np = parts(prefix_len, (long long)tiles, own_us > 0. ? fmin(us / own_us, WANT) : WANT);
   }
-  if (max_len > 0) p.ns = parts(max_len, (long long)batch * hkv * p.own_tiles);
+  if (max_len > 0) p.ns = parts(max_len, (long long)batch * hkv * p.own_tiles, WANT);
   const size_t rows_all = p.np + p.ns == 1 ? 0 : (size_t)(p.np + p.ns) * batch * hkv * g;
   p.out_bytes = (rows_all * d * 4 + 255) / 256 * 256;
   p.bytes = p.out_bytes + (rows_all * 8 + 255) / 256 * 256;
