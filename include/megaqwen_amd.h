@@ -331,6 +331,32 @@ int mq_sparse_attention(const MqPagePool* pool, const void* q, long long q_sb, l
                         long long table_stride, int width, const int* lens, int top, float scale, void* workspace,
                         size_t workspace_bytes, hipStream_t stream);
 
+/* One greedy decode step of the full model for a batch of sequences in a paged cache: batch tokens in,
+ * batch tokens out. The sequences share the prefix (as in mq_shared_prefix_attention) and have their
+ * own rows behind it; the new K and V rows go to position lens[b] of the sequence's table, whose page
+ * must be there, and lens[b] grows by one.
+ *   input_token_ids / output_token_ids: device int32 [batch], batch <= 1024.
+ *   logits_output: bf16 [batch, 151936], or NULL.
+ *   layer_weights: HOST array of pool->num_layers structs (at most 32), as for launch_prefill_float.
+ *   cos_table / sin_table: bf16 [num_positions, 128]; sequence b's position is prefix_len + lens[b].
+ *   pool: bf16, 8 kv heads of 128; its bounds are kept up if it has them.
+ *   top: 0, or the pages that each query attends to (mq_sparse_attention; prefix_len must be 0 then, the
+ *   tables hold whole sequences, and the pool needs bounds).
+ *   max_len: the longest own length that the launch is laid out for, the new row included.
+ *   workspace: 256-byte aligned, mq_decode_batch_workspace's bytes for the same arguments.
+ * On return (stream-ordered) output_token_ids[b] = argmax of the bf16 logits (lowest index on ties), or
+ * -(1 + flags) and an unchanged lens[b]: flag 1 if its id was outside the vocabulary, 2 if its position
+ * was outside the RoPE tables or its page table, 4 if it needed a page outside the pool. Uses no
+ * library workspace, allocates nothing and can be captured. */
+int mq_decode_batch(const int* input_token_ids, int* output_token_ids, void* logits_output, int batch,
+                    const void* embed_weight, const PrefillLayerWeights* layer_weights, const void* final_norm_weight,
+                    const void* lm_head_weight, const void* cos_table, const void* sin_table, int num_positions,
+                    const MqPagePool* pool, const int* prefix_pages, int prefix_len, const int* tables,
+                    long long table_stride, int width, int* lens, int max_len, int top, float attn_scale,
+                    void* workspace, size_t workspace_bytes, hipStream_t stream);
+int mq_decode_batch_workspace(const MqPagePool* pool, int batch, int prefix_len, int max_len, int top, int width,
+                              size_t* bytes);
+
 /* Human-readable name of a status code. */
 const char* mq_strerror(int status);
 

@@ -112,6 +112,10 @@ SIGNATURES = {
     # pool, q and strides, out and strides, chosen, query heads, batch, tables, table stride, width, lens,
     # top, scale, workspace, its bytes, stream
     "mq_sparse_attention": [_pool, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _i, _i, _vp, _ll, _i, _vp, _i, _f, _vp, _sz, _vp],
+    # ids, out ids, logits, batch, embed, layers (host array), final norm, lm head, cos, sin, num_positions, pool, prefix
+    # pages, prefix length, tables, table stride, width, lens, max_len, top, scale, workspace, its bytes, stream
+    "mq_decode_batch": [_vp, _vp, _vp, _i] + [_vp] * 6 + [_i, _pool, _vp, _i, _vp, _ll, _i, _vp, _i, _i, _f, _vp, _sz, _vp],
+    "mq_decode_batch_workspace": [_pool, _i, _i, _i, _i, _i, ctypes.POINTER(_sz)],
     "mq_strerror": [_i],
 }
 

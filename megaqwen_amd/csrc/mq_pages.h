@@ -51,6 +51,9 @@ struct AttnPlan {
 };
 AttnPlan plan_attention(int batch, int hkv, int g, int d, int prefix_len, int max_len);
 
+// Bytes of workspace of sparse_attention
+size_t sparse_workspace(int batch, int hkv, int g, int d, int top, int width, int page_size);
+
 // The entry points' work; len_add: rows appended since `lens` was written.
 int append_rows(const AppendArgs& A, bool f16, hipStream_t stream);
 int shared_attention(const MqPagePool* P, const void* q, int64_t q_sb, int64_t q_sh, void* out, int64_t o_sb, int64_t o_sh,

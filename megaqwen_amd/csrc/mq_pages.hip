@@ -1106,6 +1106,10 @@ int shared_attention(const MqPagePool* P, const void* q, int64_t q_sb, int64_t q
 // The chosen pages and the rows in them, ahead of the attention's partial results in the workspace.
 static size_t chosen_bytes(int batch, int hkv, int top) { return ((size_t)batch * (hkv * (size_t)top + 1) * 4 + 255) / 256 * 256; }
 
+size_t sparse_workspace(int batch, int hkv, int g, int d, int top, int width, int page_size) {
+  return chosen_bytes(batch, hkv, top) + plan_attention(batch, hkv, g, d, 0, (top < width ? top : width) * page_size).bytes;
+}
+
 int sparse_attention(const MqPagePool* P, const void* q, int64_t q_sb, int64_t q_sh, void* out, int64_t o_sb, int64_t o_sh,
                      int* chosen, int num_q_heads, int batch, const int* tables, int64_t t_sb, int width, const int* lens,
                      int len_add, int top, float scale, void* ws, size_t ws_bytes, hipStream_t stream) {

@@ -30,6 +30,7 @@
 
 #include "megaqwen_amd.h"
 #include "mq_common.h"
+#include "mq_pages.h"
 #include "mq_prefill_short.h"
 
 // Instrumentation hook of a tracing build: MQ_PF_STAMP(slot) marks a point of a kernel's
@@ -1679,6 +1680,72 @@ __global__ void __launch_bounds__(256) argmax_final(const float* bmv, const int*
   }
 }
 
+// ------------------------------------------------------------------ a decode step of a batch
+// Sequence b's embedding row, and the RoPE rows of its position (prefix_len + lens[b]) as row b of tables of
+// their own, so that the q/k/v epilogue, whose row is its position, serves a batch as it serves a prompt.
+// What is out of range reads row 0 or the last one; batch_argmax reports it.
+__global__ void __launch_bounds__(128) batch_begin(const int* ids, const uint16_t* emb, const uint16_t* cos_t,
+                                                   const uint16_t* sin_t, const int* lens, int prefix_len, int num_positions,
+                                                   uint16_t* h, uint16_t* cos_b, uint16_t* sin_b) {
+  const int b = blockIdx.x, t = threadIdx.x;
+  const int id = ids[b], len = lens[b];
+  const int at = len < 0 || len >= num_positions - prefix_len ? num_positions - 1 : prefix_len + len;
+  reinterpret_cast<u32x4*>(h + (size_t)b * H)[t] = ldw(emb + (size_t)(id < 0 || id >= VOCAB ? 0 : id) * H + 8 * t);
+  if (t < HD / 8) {
+    reinterpret_cast<u32x4*>(cos_b + (size_t)b * HD)[t] = ldw(cos_t + (size_t)at * HD + 8 * t);
+    reinterpret_cast<u32x4*>(sin_b + (size_t)b * HD)[t] = ldw(sin_t + (size_t)at * HD + 8 * t);
+  }
+}
+
+// Sequence b's greedy token (the lowest index of equal bf16 logits) and its length, one more; or -(1 + flags), and
+// the length stays: 1: its id was outside the vocabulary, 2: its position was outside the RoPE or its page table,
+// 4: its logits are not numbers (it needs a page outside the pool).
+__global__ void __launch_bounds__(1024) batch_argmax(const uint16_t* logits, const int* ids, int* lens, int prefix_len,
+                                                     int num_positions, int own_positions, int* out) {
+  __shared__ float s_v[16];
+  __shared__ int s_i[16];
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  const uint16_t* row = logits + (size_t)b * VOCAB;
+  float v = -INFINITY;
+  int i = 0x7fffffff;
+  static_assert(VOCAB % 8 == 0, "rows of 16-byte chunks");
+  for (int c = tid; c < VOCAB / 8; c += 1024) {
+    float f[8];
+    unpack8(ldw(row + 8 * c), f);
+#pragma unroll
+    for (int u = 0; u < 8; u++)
+      if (f[u] > v || (f[u] == v && 8 * c + u < i)) {
+        v = f[u];
+        i = 8 * c + u;
+      }
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    const float ov = __shfl_xor(v, off, 64);
+    const int oi = __shfl_xor(i, off, 64);
+    if (ov > v || (ov == v && oi < i)) {
+      v = ov;
+      i = oi;
+    }
+  }
+  if (lane == 0) {
+    s_v[wv] = v;
+    s_i[wv] = i;
+  }
+  __syncthreads();
+  if (tid > 0) return;
+  for (int w = 1; w < 16; w++)
+    if (s_v[w] > v || (s_v[w] == v && s_i[w] < i)) {
+      v = s_v[w];
+      i = s_i[w];
+    }
+  const int id = ids[b], len = lens[b];
+  const int flags = (id < 0 || id >= VOCAB ? 1 : 0) |
+                    (len < 0 || len >= num_positions - prefix_len || len >= own_positions ? 2 : 0) | (i == 0x7fffffff ? 4 : 0);
+  out[b] = flags ? -(1 + flags) : i;
+  if (!flags) lens[b] = len + 1;
+}
+
 }  // namespace pf
 }  // namespace mq
 
@@ -1870,6 +1937,28 @@ static void gemm_residual(GemmArgs g, hipStream_t stream) {
   }
 }
 
+// What gate/up's idle CUs read ahead for a short prompt: down_proj's weights and the next layer's
+// q/k/v and o_proj weights, each column tile on the XCD of the launch that reads it
+// (q/k/v column tiles of one head: q 0-15, k 16-23, v 24-31; the k-split residual
+// products' 64-column tiles: 16)
+static WarmSet warm_set(const PrefillLayerWeights* layer_weights, int l, int num_layers, int S) {
+  WarmSet W{};
+  if (S > WARM_MAX_S) return W;
+  auto add = [&](const void* wp, int tile_bytes, int ntiles, int xcd0) {
+    W.w[W.n] = static_cast<const uint16_t*>(wp);
+    W.tile_bytes[W.n] = tile_bytes; W.ntiles[W.n] = ntiles; W.xcd0[W.n] = xcd0; W.n++;
+  };
+  add(layer_weights[l].down_proj_weight, 64 * I * 2, H / 64, 0);
+  if (l + 1 < num_layers) {
+    const PrefillLayerWeights& wn = layer_weights[l + 1];
+    add(wn.q_proj_weight, HD * H * 2, QS / HD, 0);
+    add(wn.k_proj_weight, HD * H * 2, KVS / HD, (QS / HD) % 8);
+    add(wn.v_proj_weight, HD * H * 2, KVS / HD, (QS / HD + KVS / HD) % 8);
+    add(wn.o_proj_weight, 64 * QS * 2, H / 64, 0);
+  }
+  return W;
+}
+
 // The buffers of one prefill run, carved from a launcher's scratch arguments: the bf16
 // activations, the fp32 partial sums of the k-split o_proj and down_proj, and where the
 // last row's final norm and hidden state go (see lm_partial).
@@ -1996,24 +2085,7 @@ static int prefill_run(const int* input_token_ids, int* output_token_id, int seq
     GemmArgs gu{};
     gu.a = mln; gu.lda = H; gu.m = S; gu.k = H;
     gu.seg[0] = GemmSeg{bf(w.gate_proj_weight), bf(w.up_proj_weight), mid, 0, I};
-    WarmSet W{};
-    if (S <= WARM_MAX_S) {
-      // short prompts: the idle CUs of gate/up read down_proj's weights and the next layer's
-      // q/k/v and o_proj weights, each column tile on the XCD of the launch that reads it
-      // (q/k/v column tiles of one head: q 0-15, k 16-23, v 24-31; the k-split residual
-      // products' 64-column tiles: 16)
-      auto add = [&](const void* wp, int tile_bytes, int ntiles, int xcd0) {
-        W.w[W.n] = bf(wp); W.tile_bytes[W.n] = tile_bytes; W.ntiles[W.n] = ntiles; W.xcd0[W.n] = xcd0; W.n++;
-      };
-      add(w.down_proj_weight, 64 * I * 2, H / 64, 0);
-      if (l + 1 < num_layers) {
-        const PrefillLayerWeights& wn = layer_weights[l + 1];
-        add(wn.q_proj_weight, HD * H * 2, QS / HD, 0);
-        add(wn.k_proj_weight, HD * H * 2, KVS / HD, (QS / HD) % 8);
-        add(wn.v_proj_weight, HD * H * 2, KVS / HD, (QS / HD + KVS / HD) % 8);
-        add(wn.o_proj_weight, 64 * QS * 2, H / 64, 0);
-      }
-    }
+    const WarmSet W = warm_set(layer_weights, l, num_layers, S);
     gemm_gate_up(gu, stream, W.n > 0 ? &W : nullptr);
     chk();
     GemmArgs gd{};
@@ -2162,4 +2234,156 @@ extern "C" int launch_prefill_megakernel(const int* token_ids, int* output_token
   return prefill_run(token_ids, output_token_id, seq_len, embed_weight, layer_weights, final_norm_weight,
                      lm_head_weight, cos_table, sin_table, k_cache, v_cache, B, num_layers, max_seq_len, attn_scale,
                      stream);
+}
+
+// ------------------------------------------------------------------ a decode step of a batch
+// The sequences' tokens go through the layers as the rows of a prompt do (the same products, epilogues and
+// rounding points); only the attention differs, over the pages, and the LM head takes every row.
+constexpr int MAX_BATCH = 1024;  // (below RESADD_MIN_S)
+
+// Where a step's intermediates lie in its workspace.
+struct BatchBufs {
+  size_t h, nrm, q, k, v, att, mln, mid, parts, cos_b, sin_b, logits, chosen, attn, attn_bytes, bytes;
+};
+static BatchBufs batch_bufs(int batch, int prefix_len, int max_len, int top, int width, int page_size) {
+  BatchBufs b{};
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+  };
+  const size_t B = (size_t)batch;
+  b.h = take(B * H * 2); b.nrm = take(B * H * 2); b.q = take(B * QS * 2); b.k = take(B * KVS * 2); b.v = take(B * KVS * 2);
+  b.att = take(B * QS * 2); b.mln = take(B * H * 2); b.mid = take(B * I * 2); b.parts = take(RES_SPLIT * B * H * 4);
+  b.cos_b = take(B * HD * 2); b.sin_b = take(B * HD * 2); b.logits = take(B * VOCAB * 2);
+  b.chosen = take(top > 0 ? B * NKV * top * 4 : 0);
+  b.attn_bytes = top > 0 ? pg::sparse_workspace(batch, NKV, NQ / NKV, HD, top, width, page_size)
+                         : pg::plan_attention(batch, NKV, NQ / NKV, HD, prefix_len, max_len).bytes;
+  b.attn = take(b.attn_bytes);
+  b.bytes = at;
+  return b;
+}
+
+static bool batch_args_ok(const MqPagePool* P, int batch, int prefix_len, int max_len, int top, int width) {
+  return P && P->num_kv_heads == NKV && P->head_dim == HD && P->dtype == MQ_BF16 && P->num_layers >= 1 &&
+         P->num_layers <= MAX_LAYERS && P->page_size >= 16 && P->page_size <= 256 && (P->page_size & (P->page_size - 1)) == 0 &&
+         batch >= 1 && batch <= MAX_BATCH && prefix_len >= 0 && max_len >= 1 && top >= 0 && top <= MQ_MAX_TABLE_WIDTH &&
+         (top == 0 || (prefix_len == 0 && P->bounds)) && width >= 1 && width <= MQ_MAX_TABLE_WIDTH;
+}
+
+extern "C" int mq_decode_batch_workspace(const MqPagePool* pool, int batch, int prefix_len, int max_len, int top, int width,
+                                         size_t* bytes) {
+  if (!bytes || !batch_args_ok(pool, batch, prefix_len, max_len, top, width)) return MQ_ERR_ARG;
+  *bytes = batch_bufs(batch, prefix_len, max_len, top, width, pool->page_size).bytes;
+  return MQ_OK;
+}
+
+extern "C" int mq_decode_batch(const int* input_token_ids, int* output_token_ids, void* logits_output, int batch,
+                               const void* embed_weight, const PrefillLayerWeights* layer_weights,
+                               const void* final_norm_weight, const void* lm_head_weight, const void* cos_table,
+                               const void* sin_table, int num_positions, const MqPagePool* pool, const int* prefix_pages,
+                               int prefix_len, const int* tables, long long table_stride, int width, int* lens, int max_len,
+                               int top, float attn_scale, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  if (!batch_args_ok(pool, batch, prefix_len, max_len, top, width) || !pool->k || !pool->v || pool->num_pages < 1 || !tables ||
+      !lens || !workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || num_positions <= prefix_len || table_stride < 0 ||
+      (prefix_len > 0 && !prefix_pages) ||
+      !prefill_args_ok(input_token_ids, output_token_ids, batch, embed_weight, layer_weights, final_norm_weight, lm_head_weight,
+                       cos_table, sin_table, pool->k, pool->v, pool->num_layers, batch, attn_scale))
+    return MQ_ERR_ARG;
+  const BatchBufs B = batch_bufs(batch, prefix_len, max_len, top, width, pool->page_size);
+  if (workspace_bytes < B.bytes) return MQ_ERR_ARG;
+  char* const ws = static_cast<char*>(workspace);
+  auto bf = [](const void* p) { return static_cast<const uint16_t*>(p); };
+  auto at = [&](size_t off) { return reinterpret_cast<uint16_t*>(ws + off); };
+  uint16_t *const h = at(B.h), *const nrm = at(B.nrm), *const q = at(B.q), *const k = at(B.k), *const v = at(B.v);
+  uint16_t *const att = at(B.att), *const mln = at(B.mln), *const mid = at(B.mid);
+  uint16_t* const logits = logits_output ? static_cast<uint16_t*>(logits_output) : at(B.logits);
+  PartSet parts{};
+  parts.n = RES_SPLIT;
+  for (int z = 0; z < RES_SPLIT; z++) {
+    parts.lo[z] = reinterpret_cast<float*>(ws + B.parts) + (size_t)z * batch * H;
+    parts.hi[z] = parts.lo[z] + PART_HALF;
+    parts.ld[z] = H;
+  }
+  const int L = pool->num_layers, lp = __builtin_ctz((unsigned)pool->page_size);
+  const size_t layer = (size_t)pool->num_pages * NKV * pool->page_size * HD, bounds_layer = (size_t)pool->num_pages * NKV * 2 * HD;
+
+  hipError_t launch_err = hipSuccess;
+  auto chk = [&]() {
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess && launch_err == hipSuccess) launch_err = e;
+  };
+  (void)hipGetLastError();  // clear an error left by an unrelated earlier call
+  batch_begin<<<batch, 128, 0, stream>>>(input_token_ids, bf(embed_weight), bf(cos_table), bf(sin_table), lens, prefix_len,
+                                         num_positions, h, at(B.cos_b), at(B.sin_b));
+  chk();
+  rmsnorm_rows<<<batch, 64, 0, stream>>>(h, bf(layer_weights[0].input_layernorm_weight), nrm, batch);
+  chk();
+  for (int l = 0; l < L; l++) {
+    const PrefillLayerWeights& w = layer_weights[l];
+    GemmArgs g{};
+    g.a = nrm; g.lda = H; g.m = batch; g.k = H;
+    g.seg[0] = GemmSeg{bf(w.q_proj_weight), nullptr, nullptr, 0, QS};
+    g.seg[1] = GemmSeg{bf(w.k_proj_weight), nullptr, nullptr, 0, KVS};
+    g.seg[2] = GemmSeg{bf(w.v_proj_weight), nullptr, nullptr, 0, KVS};
+    g.qkn = QknArgs{bf(w.q_norm_weight), bf(w.k_norm_weight), at(B.cos_b), at(B.sin_b), q, k, v, batch};
+    gemm_qkv(g, stream);
+    chk();
+    MqPagePool P = *pool;
+    P.num_layers = 1;
+    P.k = static_cast<uint16_t*>(pool->k) + l * layer;
+    P.v = static_cast<uint16_t*>(pool->v) + l * layer;
+    // (bounds that only a choice of pages needs are kept up whenever the pool has them)
+    P.bounds = pool->bounds ? static_cast<uint16_t*>(pool->bounds) + l * bounds_layer : nullptr;
+    pg::AppendArgs ap{};
+    ap.k = static_cast<uint16_t*>(P.k); ap.v = static_cast<uint16_t*>(P.v); ap.bounds = static_cast<uint16_t*>(P.bounds);
+    ap.kr = k; ap.vr = v;
+    ap.k_sb = ap.v_sb = HD; ap.k_sh = ap.v_sh = (int64_t)batch * HD;
+    ap.tables = tables; ap.lens = lens; ap.t_sb = table_stride;
+    ap.num_pages = P.num_pages; ap.hkv = NKV; ap.lp = lp; ap.d = HD; ap.width = width; ap.batch = batch;
+    int st = pg::append_rows(ap, false, stream);
+    if (st != MQ_OK) return st;
+    st = top > 0 ? pg::sparse_attention(&P, q, QS, HD, att, QS, HD, reinterpret_cast<int*>(ws + B.chosen), NQ, batch, tables,
+                                        table_stride, width, lens, 1, top, attn_scale, ws + B.attn, B.attn_bytes, stream)
+                 : pg::shared_attention(&P, q, QS, HD, att, QS, HD, NQ, batch, prefix_pages, prefix_len, tables, table_stride,
+                                        width, lens, 1, max_len, attn_scale, ws + B.attn, B.attn_bytes, stream);
+    if (st != MQ_OK) return st;
+    GemmArgs go{};
+    go.a = att; go.lda = QS; go.m = batch; go.k = QS; go.part = parts;
+    go.seg[0] = GemmSeg{bf(w.o_proj_weight), nullptr, nullptr, 0, H};
+    gemm_residual(go, stream);
+    chk();
+    resid_norm_rows<RES_SPLIT><<<batch, 64, 0, stream>>>(parts, h, bf(w.post_attn_layernorm_weight), mln, batch);
+    chk();
+    GemmArgs gu{};
+    gu.a = mln; gu.lda = H; gu.m = batch; gu.k = H;
+    gu.seg[0] = GemmSeg{bf(w.gate_proj_weight), bf(w.up_proj_weight), mid, 0, I};
+    const WarmSet W = warm_set(layer_weights, l, L, batch);
+    gemm_gate_up(gu, stream, W.n > 0 ? &W : nullptr);
+    chk();
+    GemmArgs gd{};
+    gd.a = mid; gd.lda = I; gd.m = batch; gd.k = I; gd.part = parts;
+    gd.seg[0] = GemmSeg{bf(w.down_proj_weight), nullptr, nullptr, 0, H};
+    gemm_residual(gd, stream);
+    chk();
+    // then the next layer's input RMSNorm, or the final one
+    resid_norm_rows<RES_SPLIT><<<batch, 64, 0, stream>>>(
+        parts, h, bf(l + 1 < L ? layer_weights[l + 1].input_layernorm_weight : final_norm_weight), nrm, batch);
+    chk();
+  }
+  // the logits of every row: 1187 column tiles of 128, bound by the 311 MB of the LM head, which are read once
+  // for each row tile
+  static_assert(VOCAB % 128 == 0, "whole column tiles");
+  GemmArgs gl{};
+  gl.a = nrm; gl.lda = H; gl.m = batch; gl.k = H;
+  gl.seg[0] = GemmSeg{bf(lm_head_weight), nullptr, logits, VOCAB / 128, VOCAB};
+  if (batch <= 64)
+    gemm<EPI_STORE, 64, 128, 4, 1, 2, 4>(gl, VOCAB / 128, stream);
+  else
+    gemm<EPI_STORE, 128, 128, 3, 1, 4, 4>(gl, VOCAB / 128, stream);
+  chk();
+  batch_argmax<<<batch, 1024, 0, stream>>>(logits, input_token_ids, lens, prefix_len, num_positions, width << lp, output_token_ids);
+  chk();
+  return launch_err == hipSuccess ? MQ_OK : MQ_ERR_HIP;
 }

@@ -21,7 +21,7 @@ import torch
 
 from . import _abi
 from . import config as C
-from . import rope, weights
+from . import paged, rope, weights
 from .config import HEAD_DIM, HIDDEN_SIZE, INTERMEDIATE_SIZE, KV_SIZE, NUM_KV_HEADS, NUM_LAYERS, Q_SIZE, VOCAB_SIZE
 
 ATTN_SCALE = 1.0 / math.sqrt(HEAD_DIM)
@@ -407,6 +407,128 @@ class MegakernelFusedPrefillDecoder(MegakernelPrefillDecoder):
         return self.final_hidden_.to(torch.bfloat16)
 
 
+class MegakernelBatchDecoder:
+    """Decoding of several sequences at once (no counterpart in the reference, whose decoders
+    take one), beside a MegakernelPrefillDecoder whose weights, RoPE tables and prefill it uses.
+
+    Rows live in a paged cache (`cache`, a `paged.PagedKVCache`), where sequences share the pages
+    that they have in common: `prefill(ids)` makes a sequence of a prompt, `fork(seq, n)` n more that
+    go on from it, `step(seqs, tokens)` appends one token to each and returns the greedy next ones.
+    The attention reads pages that all sequences of a step begin with once for all of them; with
+    `sparse_pages` it reads, for each query, the last page and the sparse_pages - 1 others whose keys
+    could score highest. `to_decoder(seq)` hands a sequence back to the batch-1 decoder.
+
+    The pool holds `num_pages` pages of `page_size` positions (default: room for max_batch sequences of
+    the decoder's max_seq_len), 114688 bytes a position for 28 layers."""
+
+    def __init__(self, decoder: MegakernelPrefillDecoder, max_batch: int = 64, page_size: int = 64,
+                 num_pages: int | None = None, sparse_pages: int | None = None):
+        if not 1 <= max_batch <= 1024:
+            raise ValueError("max_batch must be in [1, 1024]")
+        if sparse_pages is not None and not 1 <= sparse_pages <= _abi.MQ_MAX_TABLE_WIDTH:
+            raise ValueError(f"sparse_pages must be in [1, {_abi.MQ_MAX_TABLE_WIDTH}]")
+        if page_size not in paged.PAGE_SIZES:
+            raise ValueError(f"page_size must be one of {paged.PAGE_SIZES}")
+        self.decoder = decoder
+        self.max_batch = max_batch
+        self.sparse_pages_ = sparse_pages or 0
+        per_seq = -(-decoder.max_seq_len_ // page_size)
+        self.cache = paged.PagedKVCache(num_pages or max_batch * per_seq, decoder.num_layers_, NUM_KV_HEADS, HEAD_DIM, page_size,
+                                        torch.bfloat16, decoder.embed_weight_.device, bounds=sparse_pages is not None)
+        self._key = None
+
+    def new(self) -> int:
+        return self.cache.new()
+
+    def prefill(self, input_token_ids) -> tuple[int, int]:
+        """(sequence, greedy next token) of a prompt. Runs the decoder's prefill, so that the decoder is at the
+        end of this prompt afterwards."""
+        token = self.decoder.prefill_step(input_token_ids)
+        seq = self.cache.new()
+        try:
+            self.cache.load(seq, self.decoder.k_cache_, self.decoder.v_cache_, self.decoder.position())
+        except BaseException:
+            self.cache.free(seq)
+            raise
+        return seq, token
+
+    def fork(self, seq: int, n: int = 1) -> list[int]:
+        return self.cache.fork(seq, n)
+
+    def free(self, seq: int) -> None:
+        self.cache.free(seq)
+
+    def length(self, seq: int) -> int:
+        return self.cache.length(seq)
+
+    def to_decoder(self, seq: int) -> None:
+        """The sequence's rows into the decoder's own caches: its next decode_step goes on from there."""
+        self.decoder.set_position(self.cache.store(seq, self.decoder.k_cache_, self.decoder.v_cache_))
+
+    def _prepare(self, seqs) -> None:
+        """Page tables and lengths of the sequences on the GPU, made anew when the pages or the sequences have
+        changed (the launches keep the lengths up)."""
+        cache = self.cache
+        key = (tuple(seqs), cache.version)
+        if key == self._key:
+            return
+        self._key = None
+        # (pages for a single query are its own: sharing needs two)
+        shared = cache.shared_pages(seqs) if len(seqs) > 1 and not self.sparse_pages_ else 0
+        self.tables_, self.lens_ = cache.tables(seqs, shared)
+        self.prefix_len_ = shared * cache.page_size
+        self.prefix_pages_ = torch.tensor(cache.pages(seqs[0])[:shared], dtype=torch.int32).to(self.tables_.device)
+        self._key = key
+
+    def _step(self, seqs, tokens, want_logits: bool):
+        d, cache, seqs = self.decoder, self.cache, list(seqs)
+        tokens = [int(t) for t in tokens]
+        if not 1 <= len(seqs) <= self.max_batch or len(tokens) != len(seqs):
+            raise ValueError(f"expected 1 to {self.max_batch} sequences and as many tokens")
+        if len(set(seqs)) != len(seqs):
+            raise ValueError("seqs: a sequence twice")
+        for t in tokens:
+            if not 0 <= t < VOCAB_SIZE:
+                raise ValueError(f"token id {t} out of range")
+        for s in seqs:
+            if cache.length(s) >= d.max_seq_len_:
+                raise RuntimeError("KV cache full: length >= max_seq_len")
+        cache.reserve(seqs, 1)
+        self._prepare(seqs)
+        dev, n, width = d.embed_weight_.device, len(seqs), self.tables_.shape[1]
+        pool = paged._pool(cache.k_pages, cache.v_pages, cache.bounds, True)
+        max_len = width * cache.page_size
+        lib, size = _abi.lib(), ctypes.c_size_t()
+        _abi.check(lib.mq_decode_batch_workspace(pool, n, self.prefix_len_, max_len, self.sparse_pages_, width, size),
+                   "mq_decode_batch_workspace")
+        ws = torch.empty(size.value, dtype=torch.uint8, device=dev)
+        ids = torch.tensor(tokens, dtype=torch.int32).to(dev)
+        out = torch.empty(n, dtype=torch.int32, device=dev)
+        logits = torch.empty(n, VOCAB_SIZE, dtype=torch.bfloat16, device=dev) if want_logits else None
+        paged._call("mq_decode_batch", dev, _ptr(ids), _ptr(out), _ptr(logits), n, _ptr(d.embed_weight_),
+                    ctypes.addressof(d.h_layer_weights_), _ptr(d.final_norm_weight_), _ptr(d.lm_head_weight_), _ptr(d.cos_table_),
+                    _ptr(d.sin_table_), d.cos_table_.shape[0], pool, _ptr(self.prefix_pages_) if self.prefix_len_ else None,
+                    self.prefix_len_, _ptr(self.tables_), self.tables_.stride(0), width, _ptr(self.lens_), max_len,
+                    self.sparse_pages_, d.attn_scale_, _ptr(ws), size.value)
+        got = out.tolist()
+        cache.extend([s for s, t in zip(seqs, got) if t >= 0])
+        bad = {s: -t - 1 for s, t in zip(seqs, got) if t < 0}
+        if bad:
+            self._key = None
+            raise _abi.MegakernelError(f"batch step failed for sequences {bad} (flags: 1 token id, 2 position, 4 page); "
+                                       f"their lengths are unchanged")
+        return got, logits
+
+    def step(self, seqs, tokens) -> list[int]:
+        """Appends tokens[i] to seqs[i] and returns the greedy next tokens."""
+        return self._step(seqs, tokens, False)[0]
+
+    def step_with_logits(self, seqs, tokens):
+        """step, and the bf16-rounded logits as fp32 [len(seqs), 151936]."""
+        got, logits = self._step(seqs, tokens, True)
+        return got, logits.float()
+
+
 def decode_layer(hidden_in: torch.Tensor, layer_weights: list, cos_table, sin_table, k_cache, v_cache,
                  position: int, attn_scale: float = ATTN_SCALE) -> torch.Tensor:
     """Run one decoder block on a bf16 hidden vector at `position` (C ABI `mq_decode_layer`).
@@ -727,6 +849,63 @@ class MegakernelPrefillGenerator(_GeneratorBase):
     def prefill_only(self, prompt):
         nxt = self._prefill(prompt)
         return nxt, self.decoder.position()
+
+    def _batch(self, n: int, prompt_len: int, max_new_tokens: int, sparse_pages) -> MegakernelBatchDecoder:
+        """A batch decoder with room for n continuations; the last one is kept while it is large enough."""
+        page = 64
+        each = -(-min(max_new_tokens + 1, self.max_seq_len) // page) + 1  # (the page that the prompt ends in is copied)
+        need = -(-prompt_len // page) + n * each
+        b = getattr(self, "batch_decoder_", None)
+        if b is None or b.max_batch < n or b.cache.num_pages < need or b.sparse_pages_ != (sparse_pages or 0):
+            self.batch_decoder_ = None  # (the old pool's memory first)
+            self.batch_decoder_ = b = MegakernelBatchDecoder(self.decoder, n, page, need, sparse_pages)
+        return b
+
+    def generate_many_ids(self, prompt, n: int, max_new_tokens: int = 100, stop_tokens=None, temperature: float = 1.0,
+                          do_sample: bool = False, seed=None, sparse_pages: int | None = None) -> list[list[int]]:
+        """Ids of n continuations of one prompt, decoded together: the prompt is prefilled once and its pages are
+        shared. Without do_sample all n are the greedy one. sparse_pages: see MegakernelBatchDecoder."""
+        if not 1 <= n <= 1024:
+            raise ValueError("n must be in [1, 1024]")
+        g = self._sampling(do_sample, temperature, seed)
+        ids = self._ids(prompt)
+        if not ids:
+            raise ValueError("empty prompt")
+        stop = self._stop(stop_tokens)
+        dec = self._batch(n, len(ids), max_new_tokens, sparse_pages)
+        self.decoder.reset()
+        # the last prompt token is each continuation's first step, whose logits every one samples from
+        root = dec.prefill(torch.tensor(ids[:-1], dtype=torch.int32))[0] if len(ids) > 1 else dec.new()
+        live = dict(zip(dec.fork(root, n), range(n)))
+        dec.free(root)
+        out: list[list[int]] = [[] for _ in range(n)]
+        cur = {s: ids[-1] for s in live}
+        try:
+            for _ in range(max_new_tokens):
+                if not live or dec.length(next(iter(live))) >= self.max_seq_len - 1:
+                    break
+                seqs = list(live)
+                if do_sample:
+                    _, lg = dec.step_with_logits(seqs, [cur[s] for s in seqs])
+                    nxt = [sample_next_token(row, temperature, g) for row in lg]
+                else:
+                    nxt = dec.step(seqs, [cur[s] for s in seqs])
+                for s, t in zip(seqs, nxt):
+                    if t in stop:
+                        dec.free(s)
+                        del live[s]
+                    else:
+                        out[live[s]].append(t)
+                        cur[s] = t
+        finally:
+            for s in live:
+                dec.free(s)
+        return out
+
+    def generate_many(self, prompt, n: int, max_new_tokens: int = 100, temperature: float = 1.0, stop_tokens=None,
+                      do_sample: bool = False, seed=None, sparse_pages: int | None = None):
+        return [self._detok(ids) for ids in self.generate_many_ids(prompt, n, max_new_tokens, stop_tokens, temperature, do_sample,
+                                                                  seed, sparse_pages)]
 
 
 class MegakernelFusedPrefillGenerator(MegakernelPrefillGenerator):

@@ -256,3 +256,206 @@ def sparse_attention(q, k_pages, v_pages, bounds, tables, lens, top_pages: int, 
     _call("mq_sparse_attention", k_pages.device, pool, q.data_ptr(), q_sb, q_sh, out.data_ptr(), o_sb, o_sh, chosen.data_ptr(), heads,
           batch, tables.data_ptr(), t_sb, width, lens.data_ptr(), top, _scale(scale, pool.head_dim), ws.data_ptr(), ws_bytes)
     return out, chosen
+
+
+class PagedKVCache:
+    """The books of a page pool: sequences as lists of pages, shared until one of them writes.
+
+    Sequences are numbers that `new`, `fork` and `free` hand out and take back. `fork` copies nothing: the
+    new sequences use the same pages, and `reserve` gives a sequence a page of its own (a copy of the
+    last one, if it is shared and not full) before a row is appended. `compact` moves the pages in
+    use to the front of the pool.
+
+    `k_pages`, `v_pages` `[layers, pages, kv heads, page size, head dim]` and, with `bounds=True`, `bounds`
+    (for `sparse_attention`) are the pool; the functions of this module take them, or one layer of
+    them. Rows that were appended by `append_rows` are made known with `extend`. A pool without a free
+    page raises MegakernelError, before anything has changed."""
+
+    def __init__(self, num_pages: int, num_layers: int = NUM_LAYERS, num_kv_heads: int = NUM_KV_HEADS, head_dim: int = HEAD_DIM,
+                 page_size: int = 64, dtype=torch.bfloat16, device="cuda", bounds: bool = False):
+        if dtype not in _DTYPES:
+            raise ValueError(f"dtype: expected bfloat16 or float16, got {dtype}")
+        if page_size not in PAGE_SIZES or head_dim not in HEAD_DIMS:
+            raise ValueError(f"page size {page_size} (of {PAGE_SIZES}) or head dim {head_dim} (of {HEAD_DIMS})")
+        if min(num_pages, num_layers, num_kv_heads) < 1:
+            raise ValueError("num_pages, num_layers and num_kv_heads must be positive")
+        shape = (num_layers, num_pages, num_kv_heads, page_size, head_dim)
+        self.page_size, self.num_pages = page_size, num_pages
+        self.k_pages = torch.zeros(shape, dtype=dtype, device=device)
+        self.v_pages = torch.zeros(shape, dtype=dtype, device=device)
+        self.bounds = torch.zeros(shape[:3] + (2, head_dim), dtype=dtype, device=device) if bounds else None
+        self._free = list(range(num_pages))  # a heap: the lowest page first
+        self._users = [0] * num_pages
+        self._seqs: dict[int, list] = {}  # sequence -> [pages, rows]
+        self._next = 0
+        self.version = 0  # changes with every change of a page list
+
+    # -- the books ---------------------------------------------------------------
+    def _of(self, seq: int) -> list:
+        try:
+            return self._seqs[seq]
+        except KeyError:
+            raise ValueError(f"no sequence {seq}") from None
+
+    def _take(self, n: int) -> list[int]:
+        if n > len(self._free):
+            raise _abi.MegakernelError(f"page pool exhausted: {n} pages wanted, {len(self._free)} of {self.num_pages} free")
+        pages = [heapq.heappop(self._free) for _ in range(n)]
+        for p in pages:
+            self._users[p] = 1
+        return pages
+
+    def _drop(self, pages) -> None:
+        for p in pages:
+            self._users[p] -= 1
+            if self._users[p] == 0:
+                heapq.heappush(self._free, p)
+
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def pages(self, seq: int) -> list[int]:
+        return list(self._of(seq)[0])
+
+    def length(self, seq: int) -> int:
+        return self._of(seq)[1]
+
+    def new(self) -> int:
+        """A sequence without rows."""
+        seq, self._next = self._next, self._next + 1
+        self._seqs[seq] = [[], 0]
+        return seq
+
+    def fork(self, seq: int, n: int = 1) -> list[int]:
+        """n sequences with the rows of `seq`, whose pages they share. No row is copied."""
+        pages, rows = self._of(seq)
+        if n < 0:
+            raise ValueError("n must not be negative")
+        out = []
+        for _ in range(n):
+            s = self.new()
+            self._seqs[s] = [list(pages), rows]
+            out.append(s)
+        for p in pages:
+            self._users[p] += n
+        return out
+
+    def free(self, seq: int) -> None:
+        """Gives the sequence's pages back, those that no other sequence uses to the pool."""
+        pages, _ = self._of(seq)
+        del self._seqs[seq]
+        self._drop(pages)
+        self.version += 1
+
+    def reserve(self, seqs, rows: int = 1) -> None:
+        """Makes room for `rows` more rows behind each sequence: new pages, and a copy of a last page that
+        others use too and that is not full (one launch for all of them)."""
+        if rows < 0:
+            raise ValueError("rows must not be negative")
+        seqs = list(seqs)
+        if len(set(seqs)) != len(seqs):
+            raise ValueError("seqs: a sequence twice")
+        users, plan, want = {}, [], 0
+        for s in seqs:
+            pages, n = self._of(s)
+            more = max(0, -(-(n + rows) // self.page_size) - len(pages))
+            own = False
+            if rows and n % self.page_size:
+                last = pages[n // self.page_size]
+                left = users.get(last, self._users[last])
+                own = left > 1
+                users[last] = left - own
+            plan.append((pages, n, more, own))
+            want += more + own
+        if not want:
+            return
+        taken = iter(self._take(want))
+        src, dst = [], []
+        for pages, n, more, own in plan:
+            if own:
+                at = n // self.page_size
+                src.append(pages[at])
+                dst.append(next(taken))
+                self._users[pages[at]] -= 1
+                pages[at] = dst[-1]
+            pages.extend(next(taken) for _ in range(more))
+        self.version += 1
+        if src:
+            copy_pages(self.k_pages, self.v_pages, src, dst, bounds=self.bounds)
+
+    def extend(self, seqs, rows: int = 1) -> None:
+        """`rows` rows were appended to each sequence (within what `reserve` made room for)."""
+        seqs = list(seqs)
+        for s in seqs:
+            pages, n = self._of(s)
+            if not 0 <= n + rows <= len(pages) * self.page_size or rows < 0:
+                raise ValueError(f"sequence {s}: {n} + {rows} rows do not fit its {len(pages)} pages")
+        for s in seqs:
+            self._seqs[s][1] += rows
+
+    def load(self, seq: int, k_cache, v_cache, length: int) -> None:
+        """Rows 0 .. length - 1 of contiguous caches as all of the sequence's rows (it has none yet)."""
+        pages, n = self._of(seq)
+        if pages or n:
+            raise ValueError(f"sequence {seq} has rows already")
+        if length < 0:
+            raise ValueError("length must not be negative")
+        taken = self._take(-(-length // self.page_size))
+        try:
+            load_pages(k_cache, v_cache, self.k_pages, self.v_pages, taken, length, bounds=self.bounds)
+        except BaseException:
+            self._drop(taken)
+            raise
+        self._seqs[seq] = [taken, length]
+        self.version += 1
+
+    def store(self, seq: int, k_cache, v_cache) -> int:
+        """The sequence's rows into contiguous caches, from position 0; returns how many."""
+        pages, n = self._of(seq)
+        store_pages(self.k_pages, self.v_pages, pages[: -(-n // self.page_size)], n, k_cache, v_cache)
+        return n
+
+    def compact(self) -> int:
+        """Moves the pages in use to the front of the pool, one launch; returns their number. Page lists are
+        rewritten; tables made before are void."""
+        used = [p for p, u in enumerate(self._users) if u]
+        src = [p for p in used if p >= len(used)]
+        if not src:
+            return len(used)
+        dst = [p for p in range(len(used)) if not self._users[p]]
+        copy_pages(self.k_pages, self.v_pages, src, dst, bounds=self.bounds)
+        to = dict(zip(src, dst))
+        for entry in self._seqs.values():
+            entry[0] = [to.get(p, p) for p in entry[0]]
+        for a, b in to.items():
+            self._users[b], self._users[a] = self._users[a], 0
+        self._free = list(range(len(used), self.num_pages))
+        self.version += 1
+        return len(used)
+
+    # -- what the attentions read --------------------------------------------------
+    def shared_pages(self, seqs) -> int:
+        """How many pages all of the sequences begin with, full in every one of them."""
+        lists = [self._of(s) for s in seqs]
+        if not lists:
+            return 0
+        most = min(n for _, n in lists) // self.page_size
+        first = lists[0][0]
+        for at in range(most):
+            if any(pages[at] != first[at] for pages, _ in lists):
+                return at
+        return most
+
+    def tables(self, seqs, first: int = 0):
+        """(tables, lens) of the sequences on the GPU, int32 `[n, width]` and `[n]`, from their page number `first` on:
+        all pages they have, room that was reserved included, and the rows in them so far."""
+        lists = [self._of(s) for s in seqs]
+        if not lists:
+            raise ValueError("seqs: expected at least one sequence")
+        width = max(1, max(len(pages) - first for pages, _ in lists))
+        if width > _abi.MQ_MAX_TABLE_WIDTH:
+            raise ValueError(f"a sequence of {width} pages exceeds the table width {_abi.MQ_MAX_TABLE_WIDTH}")
+        table = [pages[first:] + [-1] * (width - max(0, len(pages) - first)) for pages, _ in lists]
+        lens = [max(0, n - first * self.page_size) for _, n in lists]
+        device = self.k_pages.device
+        return torch.tensor(table, dtype=torch.int32).to(device), torch.tensor(lens, dtype=torch.int32).to(device)

@@ -198,3 +198,234 @@ def test_attention_refusals():
     _refused("bounds", sparse, Q, k, k, b[:4], T, LENS, 2)
     _refused("on the GPU", shared, Q, k, k, pre, 20, T, LENS)
     _refused("on the GPU", sparse, Q, k, k, b, T, LENS, 2)
+
+
+# ---------------------------------------------------------------- the batched decode step
+
+def _layers(n=2, **over):
+    arr = (_abi.LDGLayerWeights * n)()
+    for i in range(n):
+        for name in _abi.LAYER_FIELDS:
+            setattr(arr[i], name, over.get(name, 16))
+    return arr
+
+
+def _batch(pool=None, made=None, **over):
+    made = _layers() if made is None else made
+    a = dict(ids=16, out=16, logits=None, batch=3, embed=16, layers=ctypes.addressof(made), norm=16, lm=16, cos=16, sin=16,
+             num_positions=100, pool=pool or _model_pool(), prefix_pages=16, prefix_len=64, tables=16, t_sb=4, width=4, lens=16,
+             max_len=64, top=0, scale=0.1, ws=256, ws_bytes=1 << 40)
+    a.update(over)
+    return _abi.lib().mq_decode_batch(*a.values(), None)
+
+
+def _model_pool(**over):
+    return _pool(**{**dict(num_layers=2, num_kv_heads=8, page_size=64, head_dim=128), **over})
+
+
+@pytest.mark.parametrize("bad", [
+    dict(ids=None), dict(out=None), dict(batch=0), dict(batch=1025), dict(embed=None), dict(layers=None), dict(norm=None), dict(lm=None),
+    dict(cos=None), dict(sin=None), dict(num_positions=64), dict(prefix_pages=None), dict(prefix_len=-1), dict(tables=None), dict(t_sb=-1),
+    dict(width=0), dict(width=8193), dict(lens=None), dict(max_len=0), dict(top=-1), dict(top=4), dict(scale=0.0), dict(scale=float("nan")),
+    dict(ws=None), dict(ws=128), dict(ws_bytes=1000), dict(pool=_model_pool(num_kv_heads=4)), dict(pool=_model_pool(head_dim=64)),
+    dict(pool=_model_pool(dtype=_abi.MQ_FP16)), dict(pool=_model_pool(num_layers=33)), dict(pool=_model_pool(page_size=24)),
+    dict(pool=_model_pool(k=None)), dict(pool=_model_pool(num_pages=0)), dict(pool=_model_pool(bounds=None), top=4, prefix_len=0)], ids=str)
+def test_decode_batch_refuses(bad):
+    assert _batch(**bad) == _abi.MQ_ERR_ARG
+
+
+def test_decode_batch_refuses_a_missing_weight():
+    assert _batch(made=_layers(down_proj_weight=None)) == _abi.MQ_ERR_ARG
+
+
+def test_decode_batch_workspace_query():
+    L, n = _abi.lib(), ctypes.c_size_t()
+    for bad in ((_model_pool(num_kv_heads=2), 3, 0, 64, 0, 4), (_model_pool(), 0, 0, 64, 0, 4), (_model_pool(), 3, 64, 64, 4, 4),
+                (_model_pool(), 3, 0, 0, 0, 4), (_model_pool(), 3, 0, 64, 0, 0)):
+        assert L.mq_decode_batch_workspace(*bad, n) == _abi.MQ_ERR_ARG
+    assert L.mq_decode_batch_workspace(_model_pool(), 3, 640, 64, 0, 4, n) == _abi.MQ_OK
+    assert n.value >= 3 * 151936 * 2
+
+
+# ---------------------------------------------------------------- the books
+
+@pytest.fixture
+def cpu_pages(monkeypatch):
+    """The page moves on the CPU, so that the books can be checked without a GPU."""
+    def copy(k, v, src, dst, bounds=None):
+        assert len(src) == len(dst) and len(set(dst)) == len(dst) and not set(src) & set(dst)
+        for t in (k, v):
+            t[:, dst] = t[:, src].clone()
+
+    def load(kc, vc, k, v, pages, length, bounds=None):
+        for t, c in ((k, kc), (v, vc)):
+            for i in range(length):
+                t[:, pages[i // t.shape[3]], :, i % t.shape[3]] = c[:, :, i]
+
+    def store(k, v, pages, length, kc, vc):
+        for t, c in ((k, kc), (v, vc)):
+            for i in range(length):
+                c[:, :, i] = t[:, pages[i // t.shape[3]], :, i % t.shape[3]]
+
+    monkeypatch.setattr(paged, "copy_pages", copy)
+    monkeypatch.setattr(paged, "load_pages", load)
+    monkeypatch.setattr(paged, "store_pages", store)
+
+
+def _cache(num_pages=40, page_size=16):
+    return paged.PagedKVCache(num_pages, 1, 1, 64, page_size, torch.bfloat16, "cpu")
+
+
+def _grow(cache, seqs, values):
+    """What append_rows does to position length(seq)."""
+    cache.reserve(seqs)
+    for s, x in zip(seqs, values):
+        n, p = cache.length(s), cache.page_size
+        cache.k_pages[0, cache.pages(s)[n // p], 0, n % p, 0] = x
+    cache.extend(seqs)
+
+
+def _rows(cache, seq):
+    kc, vc = torch.zeros(1, 1, 400, 64, dtype=BF), torch.zeros(1, 1, 400, 64, dtype=BF)
+    n = cache.store(seq, kc, vc)
+    assert n == cache.length(seq)
+    return kc[0, 0, :n, 0].tolist()
+
+
+def _check_books(cache):
+    users = [0] * cache.num_pages
+    for pages, n in cache._seqs.values():
+        assert len(set(pages)) == len(pages) and n <= len(pages) * cache.page_size
+        for p in pages:
+            users[p] += 1
+    assert users == cache._users
+    assert sorted(cache._free) == [p for p, u in enumerate(users) if u == 0]
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_cache_against_plain_lists(cpu_pages, seed):
+    """Random forks, appends, frees and compactions; every sequence's rows are those of a list of its own."""
+    import random
+
+    rng = random.Random(seed)
+    cache, plain = _cache(), {}
+    root = cache.new()
+    plain[root] = []
+    for step in range(300):
+        op = rng.choice(["append", "append", "append", "append", "fork", "free", "compact"])
+        live = list(plain)
+        if op == "append" and live:
+            seqs = rng.sample(live, rng.randint(1, len(live)))
+            values = [float(rng.randint(-128, 128)) for _ in seqs]
+            try:
+                _grow(cache, seqs, values)
+            except _abi.MegakernelError:
+                _check_books(cache)  # (nothing has changed)
+                victim = rng.choice(live)
+                cache.free(victim)
+                del plain[victim]
+            else:
+                for s, x in zip(seqs, values):
+                    plain[s].append(x)
+        elif op == "fork" and live and len(live) < 9:
+            s, n = rng.choice(live), rng.randint(0, 3)
+            for t in cache.fork(s, n):
+                plain[t] = list(plain[s])
+        elif op == "free" and len(live) > 3:
+            s = rng.choice(live)
+            cache.free(s)
+            del plain[s]
+        elif op == "compact":
+            used = cache.compact()
+            assert used == cache.num_pages - cache.free_pages() and sorted(cache._free) == list(range(used, cache.num_pages))
+        _check_books(cache)
+        for s, rows in plain.items():
+            assert _rows(cache, s) == rows
+    for s in list(plain):
+        cache.free(s)
+    assert cache.free_pages() == cache.num_pages
+
+
+def test_fork_copies_a_page_only_when_it_is_written(cpu_pages):
+    cache = _cache()
+    kc = torch.arange(40, dtype=torch.float32).view(1, 1, 40, 1).expand(1, 1, 40, 64).to(BF).contiguous()
+    a = cache.new()
+    cache.load(a, kc, kc, 20)  # two pages, the second with 4 rows
+    assert cache.pages(a) == [0, 1] and cache.free_pages() == 38
+    b, c = cache.fork(a, 2)
+    assert cache.pages(b) == cache.pages(c) == [0, 1] and cache.free_pages() == 38
+    assert cache.shared_pages([a, b, c]) == 1  # (the full one)
+    _grow(cache, [a, b, c], [100.0, 101.0, 102.0])
+    # two of the three copied their last page, the last one kept it; the first stays shared
+    assert sorted(cache.pages(s)[1] for s in (a, b, c)) == [1, 2, 3] and all(cache.pages(s)[0] == 0 for s in (a, b, c))
+    for s, x in ((a, 100.0), (b, 101.0), (c, 102.0)):
+        assert _rows(cache, s) == [float(i) for i in range(20)] + [x]
+    cache.free(a)
+    cache.free(b)
+    assert _rows(cache, c)[-1] == 102.0 and cache.free_pages() == 38
+
+
+def test_a_full_shared_page_is_not_copied(cpu_pages):
+    cache = _cache()
+    a = cache.new()
+    for i in range(32):
+        _grow(cache, [a], [float(i)])
+    assert cache.pages(a) == [0, 1]
+    b = cache.fork(a)[0]
+    _grow(cache, [a, b], [1.0, 2.0])
+    assert cache.pages(a)[:2] == cache.pages(b)[:2] == [0, 1] and cache.pages(a)[2] != cache.pages(b)[2]
+    assert cache.shared_pages([a, b]) == 2 and cache.shared_pages([a]) == 2
+
+
+def test_tables_of_a_batch(cpu_pages):
+    cache = _cache()
+    a = cache.new()
+    for i in range(35):
+        _grow(cache, [a], [float(i)])
+    b = cache.fork(a)[0]
+    _grow(cache, [b], [1.0])
+    for _ in range(14):
+        _grow(cache, [b], [1.0])
+    tables, lens = cache.tables([a, b], first=2)
+    assert lens.tolist() == [3, 18] and tables.shape == (2, 2) and tables.dtype == torch.int32
+    assert tables[0].tolist() == [cache.pages(a)[2], -1] and tables[1].tolist() == cache.pages(b)[2:]
+    whole, lens = cache.tables([a])
+    assert lens.tolist() == [35] and whole[0].tolist() == cache.pages(a)
+    empty, lens = cache.tables([cache.new()])
+    assert lens.tolist() == [0] and empty.tolist() == [[-1]]
+
+
+def test_cache_refusals(cpu_pages):
+    for bad in (dict(num_pages=0), dict(num_pages=4, page_size=24), dict(num_pages=4, head_dim=80), dict(num_pages=4, dtype=torch.float32),
+                dict(num_pages=4, num_layers=0)):
+        with pytest.raises(ValueError):
+            paged.PagedKVCache(device="cpu", **bad)
+    cache = _cache(num_pages=2)
+    a = cache.new()
+    for call in (lambda: cache.free(99), lambda: cache.fork(99), lambda: cache.fork(a, -1), lambda: cache.reserve([a, a]),
+                 lambda: cache.reserve([a], -1), lambda: cache.extend([a], 1), lambda: cache.length(99), lambda: cache.tables([]),
+                 lambda: cache.load(a, CACHE, CACHE, -1)):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(_abi.MegakernelError, match="exhausted"):
+        cache.reserve([a], 33)
+    assert cache.pages(a) == [] and cache.free_pages() == 2
+    kc = torch.zeros(1, 1, 40, 64, dtype=BF)
+    with pytest.raises(_abi.MegakernelError, match="exhausted"):
+        cache.load(a, kc, kc, 33)
+    cache.load(a, kc, kc, 32)
+    with pytest.raises(ValueError, match="has rows"):
+        cache.load(a, kc, kc, 1)
+    cache.free(a)
+    with pytest.raises(ValueError):
+        cache.free(a)
+    assert cache.free_pages() == 2
+
+
+def test_a_failed_load_gives_its_pages_back():
+    cache = _cache(num_pages=4)  # (the real load_pages, which refuses CPU tensors)
+    a = cache.new()
+    kc = torch.zeros(1, 1, 40, 64, dtype=BF)
+    with pytest.raises(ValueError, match="on the GPU"):
+        cache.load(a, kc, kc, 20)
+    assert cache.free_pages() == 4 and cache.pages(a) == [] and cache.length(a) == 0
