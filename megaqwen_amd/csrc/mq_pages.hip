@@ -252,8 +252,9 @@ struct Pages {
   const int* table;
   int first, last, ids, num_pages;
   bool bad;  // an id was outside the pool (page 0 is read in its place)
-  __device__ __forceinline__ Pages(const int* t, int n, int page_lo, int page_last, int lane)
-      : table(t), first(page_lo), last(page_last), num_pages(n), bad(false) {
+  __device__ __forceinline__ Pages(const int* t, int n, int page_lo, int page_last, int lane, bool any)
+      : table(t), first(page_lo), last(page_last), ids(0), num_pages(n), bad(false) {
+    if (!any) return;  // (a run without keys may have no table)
     ids = *(gint*)(table + min(first + lane, last));
     settled(ids);
   }
@@ -446,12 +447,19 @@ __device__ __forceinline__ void store_o(const AttnArgs& A, int slot, int h, int 
   if (d0 == 0) A.part_ml[at] = make_float2(m, l);
 }
 
-// Keys [k_lo, k_hi) of `table` for up to RB * 16 query rows. The waves take 32-key steps in turn and do not
-// wait for each other until the end: each has 16 KB of LDS, half for K and half for V, and asks for the next
-// step's K as soon as it has the scores of this one, for its V once this one's is multiplied.
-template <bool F16, int D, int RB>
-__device__ __forceinline__ void own_part(const AttnArgs& A, const int* table, int h, int b0, int row0, int rows, int k_lo, int k_hi,
-                                         int slot, uint32_t lds, float (*s_m)[64], float (*s_l)[64]) {
+// A run of keys: positions [lo, hi) of the sequence (or prefix) with page table `table`
+struct Run {
+  const int* table;
+  int lo, hi;
+};
+
+// The keys of N runs for up to RB * 16 query rows. The waves take 32-key steps in turn and do not wait for each
+// other until the end: each has 16 KB of LDS, half for K and half for V, and asks for the next step's K as soon as
+// it has the scores of this one, for its V once this one's is multiplied. The rows are read once
+// (or, of several runs, by few workgroups), past the caches: non-temporal, 6.1 against 5.4 TB/s.
+template <bool F16, int D, int RB, int N>
+__device__ __forceinline__ void own_part(const AttnArgs& A, const Run (&runs)[N], int h, int b0, int row0, int rows, int slot,
+                                         uint32_t lds, float (*s_m)[64], float (*s_l)[64]) {
   constexpr uint32_t HALF = KS * D * 2, WAVE = 2 * HALF;  // bytes of a step's K (or V), and of a wave
   constexpr int NI = KS * D * 2 / 1024;                   // DMA instructions of a step's K (or V)
   static_assert(RB * 16 * D * 4 <= (int)WAVE, "a wave's output fits its LDS");
@@ -459,24 +467,7 @@ __device__ __forceinline__ void own_part(const AttnArgs& A, const int* table, in
   const int pmask = (1 << A.lp) - 1;
   const size_t page_elems = ((size_t)A.hkv << A.lp) * D, head_elems = ((size_t)h << A.lp) * D;
   const uint32_t mine = lds + WAVE * wv;
-  Pages pages(table, A.num_pages, k_lo >> A.lp, (k_hi - 1) >> A.lp, lane);
-  size_t base[2];  // the pages of a step's two 16-key halves
-  auto find = [&](int k0) {
-    base[0] = (size_t)pages(k0 >> A.lp, lane) * page_elems + head_elems;
-    base[1] = A.lp == 4 && k0 + 16 < k_hi ? (size_t)pages((k0 >> 4) + 1, lane) * page_elems + head_elems : base[0];
-  };
-  auto fetch = [&](const uint16_t* pool, int k0, uint32_t dst) {
-    fetch16<D, true>(pool, base[0], k0, k_hi - 1, pmask, dst, lane);
-    fetch16<D, true>(pool, base[1], k0 + 16, k_hi - 1, pmask, dst + HALF / 2, lane);
-  };
-  int k0 = k_lo + KS * wv;
-  if (k0 < k_hi) {
-    find(k0);
-    fetch(A.k, k0, mine);
-    fetch(A.v, k0, mine + HALF);
-  }
   u32x4 qf[RB][D / 32];
-  load_q<D, RB>(A, h, b0, row0, rows, r16, kg, qf);
   float m[RB];
   f32x4 l[RB], o[RB][D / 16];
 #pragma unroll
@@ -487,21 +478,45 @@ __device__ __forceinline__ void own_part(const AttnArgs& A, const int* table, in
     for (int dt = 0; dt < D / 16; dt++) o[rb][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   const uint32_t ka = k_frag<D>(r16, kg), va = v_frag<D>(r16, kg);
-  for (; k0 < k_hi; k0 += KS * AW) {
-    const int next = k0 + KS * AW;
-    PG_AWAIT(NI);  // K is there (V may be in flight)
-    attend_step<F16, D, RB, KS / 16>(mine, mine + HALF, k_hi - k0, A.scale_log2, kg, ka, va, qf, m, l, o, [&] {
-      PG_READ();  // (K is in registers)
-      if (next < k_hi) {
-        find(next);
-        fetch(A.k, next, mine);
-        PG_AWAIT(NI);  // V is there (the next K may be in flight)
-      } else {
-        PG_AWAIT(0);
-      }
-    });
-    PG_READ();
-    if (next < k_hi) fetch(A.v, next, mine + HALF);
+  bool bad = false;
+#pragma unroll
+  for (int n = 0; n < N; n++) {
+    const int k_hi = runs[n].hi;
+    int k0 = runs[n].lo + KS * wv;
+    const bool any = k0 < k_hi;  // (the wave's)
+    Pages pages(runs[n].table, A.num_pages, runs[n].lo >> A.lp, max(runs[n].lo, k_hi - 1) >> A.lp, lane, any);
+    size_t base[2];  // the pages of a step's two 16-key halves
+    auto find = [&](int k0) {
+      base[0] = (size_t)pages(k0 >> A.lp, lane) * page_elems + head_elems;
+      base[1] = A.lp == 4 && k0 + 16 < k_hi ? (size_t)pages((k0 >> 4) + 1, lane) * page_elems + head_elems : base[0];
+    };
+    auto fetch = [&](const uint16_t* pool, int k0, uint32_t dst) {
+      fetch16<D, true>(pool, base[0], k0, k_hi - 1, pmask, dst, lane);
+      fetch16<D, true>(pool, base[1], k0 + 16, k_hi - 1, pmask, dst + HALF / 2, lane);
+    };
+    if (any) {
+      find(k0);
+      fetch(A.k, k0, mine);
+      fetch(A.v, k0, mine + HALF);
+    }
+    if (n == 0) load_q<D, RB>(A, h, b0, row0, rows, r16, kg, qf);
+    for (; k0 < k_hi; k0 += KS * AW) {
+      const int next = k0 + KS * AW;
+      PG_AWAIT(NI);  // K is there (V may be in flight)
+      attend_step<F16, D, RB, KS / 16>(mine, mine + HALF, k_hi - k0, A.scale_log2, kg, ka, va, qf, m, l, o, [&] {
+        PG_READ();  // (K is in registers)
+        if (next < k_hi) {
+          find(next);
+          fetch(A.k, next, mine);
+          PG_AWAIT(NI);  // V is there (the next K may be in flight)
+        } else {
+          PG_AWAIT(0);
+        }
+      });
+      PG_READ();
+      if (next < k_hi) fetch(A.v, next, mine + HALF);
+    }
+    bad |= pages.bad;
   }
   // ---- join the waves: each scales its output to the rows' common maximum and leaves it in its LDS (row:
   // D / 4 pieces of 16 bytes, swizzled with the row), then all add the four up
@@ -509,7 +524,7 @@ __device__ __forceinline__ void own_part(const AttnArgs& A, const int* table, in
   for (int rb = 0; rb < RB; rb++) {
     if (kg == 0) {
       s_m[wv][16 * rb + r16] = m[rb];
-      s_l[wv][16 * rb + r16] = pages.bad ? NAN : l[rb][0];
+      s_l[wv][16 * rb + r16] = bad ? NAN : l[rb][0];
     }
   }
   __syncthreads();
@@ -558,7 +573,7 @@ __device__ __forceinline__ void prefix_part(const AttnArgs& A, int h, int row0, 
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, kg = lane >> 4;
   const int pmask = (1 << A.lp) - 1;
   const size_t page_elems = ((size_t)A.hkv << A.lp) * D, head_elems = ((size_t)h << A.lp) * D;
-  Pages pages(A.prefix_pages, A.num_pages, k_lo >> A.lp, (k_hi - 1) >> A.lp, lane);
+  Pages pages(A.prefix_pages, A.num_pages, k_lo >> A.lp, (k_hi - 1) >> A.lp, lane, true);
   // wave w brings keys 16 w .. + 15 of a step; a step's first page past the end is its last key's
   auto fetch = [&](int k0, uint32_t dst) {
     const int k = min(k0 + 16 * wv, k_hi - 1);
@@ -603,8 +618,9 @@ constexpr int UNIT = KS * AW;
 __host__ __device__ __forceinline__ int part_keys(int len, int parts) { return ((len + parts - 1) / parts + UNIT - 1) / UNIT * UNIT; }
 
 // How the query rows of a prefix are tiled: up to 32 rows, all keys' work is split among the waves (own_part);
-// more rows are (prefix_part).
-enum : int { ROWS16 = 0, ROWS32 = 1, ROWS64 = 2, ROWS128 = 3 };
+// more rows are (prefix_part). JOINED: no tiles of the prefix; each sequence's workgroup goes over the prefix and
+// then over its own rows, so that nothing is left to join and the call is one launch.
+enum : int { ROWS16 = 0, ROWS32 = 1, ROWS64 = 2, ROWS128 = 3, JOINED = 4 };
 __host__ __device__ constexpr int tile_rows(int form) { return 16 << form; }
 
 template <bool F16, int D, int FORM>
@@ -613,37 +629,47 @@ __global__ void __launch_bounds__(64 * AW, 2) attn_kernel(AttnArgs A) {
   __shared__ float s_m[AW][64], s_l[AW][64];
   static_assert(sizeof(s_kv) == AW * 2 * KS * D * 2, "the two forms take the same LDS");
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&s_kv[0];
-  // parts of the prefix and of own rows alternate, a workgroup a CU of each, while there are both
-  const int n_prefix = A.hkv * A.prefix_tiles * A.np, n_own = A.hkv * A.own_tiles * A.batch * A.ns;
-  const int runs = min(n_prefix, n_own) / NUM_CUS, bid = blockIdx.x, run = bid / NUM_CUS, rest = bid - runs * NUM_CUS;
-  const bool prefix = run < 2 * runs ? run % 2 == 0 : rest < n_prefix;
-  int id = run < 2 * runs ? run / 2 * NUM_CUS + bid % NUM_CUS : rest < n_prefix ? rest : bid - n_prefix;
-  const int h = id % A.hkv;  // (fastest: with 8 kv heads each XCD reads one head's rows)
-  id /= A.hkv;
-  if (prefix) {
-    const int rows = A.batch * A.g, row0 = tile_rows(FORM) * (id % A.prefix_tiles), part = id / A.prefix_tiles;
-    const int ch = part_keys(A.prefix_len, A.np), lo = part * ch, hi = min(A.prefix_len, lo + ch);
-    if constexpr (FORM <= ROWS32)
-      own_part<F16, D, FORM == ROWS16 ? 1 : 2>(A, A.prefix_pages, h, 0, row0, rows, lo, hi, part, lds, s_m, s_l);
-    else
-      prefix_part<F16, D, FORM == ROWS64 ? 1 : 2>(A, h, row0, rows, lo, hi, part, lds);
-    return;
+  if constexpr (FORM == JOINED) {
+    const int h = blockIdx.x % A.hkv, id = blockIdx.x / A.hkv, tile = id % A.own_tiles, b = id / A.own_tiles;
+    const int len = max(0, min(A.lens[b] + A.len_add, A.width << A.lp));
+    const Run runs[2] = {{A.prefix_pages, 0, A.prefix_len}, {A.tables + (size_t)b * A.t_sb + (size_t)h * A.t_sh, 0, len}};
+    own_part<F16, D, 1>(A, runs, h, b, 16 * tile, A.g, 0, lds, s_m, s_l);
+  } else {
+    // parts of the prefix and of own rows alternate, a workgroup a CU of each, while there are both
+    const int n_prefix = A.hkv * A.prefix_tiles * A.np, n_own = A.hkv * A.own_tiles * A.batch * A.ns;
+    const int runs = min(n_prefix, n_own) / NUM_CUS, bid = blockIdx.x, run = bid / NUM_CUS, rest = bid - runs * NUM_CUS;
+    const bool prefix = run < 2 * runs ? run % 2 == 0 : rest < n_prefix;
+    int id = run < 2 * runs ? run / 2 * NUM_CUS + bid % NUM_CUS : rest < n_prefix ? rest : bid - n_prefix;
+    const int h = id % A.hkv;  // (fastest: with 8 kv heads each XCD reads one head's rows)
+    id /= A.hkv;
+    if (prefix) {
+      const int rows = A.batch * A.g, row0 = tile_rows(FORM) * (id % A.prefix_tiles), part = id / A.prefix_tiles;
+      const int ch = part_keys(A.prefix_len, A.np), lo = part * ch, hi = min(A.prefix_len, lo + ch);
+      if constexpr (FORM <= ROWS32) {
+        const Run mine[1] = {{A.prefix_pages, lo, hi}};
+        own_part<F16, D, FORM == ROWS16 ? 1 : 2>(A, mine, h, 0, row0, rows, part, lds, s_m, s_l);
+      } else {
+        prefix_part<F16, D, FORM == ROWS64 ? 1 : 2>(A, h, row0, rows, lo, hi, part, lds);
+      }
+      return;
+    }
+    const int tile = id % A.own_tiles;
+    id /= A.own_tiles;
+    const int b = id % A.batch, part = id / A.batch;
+    const int len = max(0, min(A.lens[b] + A.len_add, A.width << A.lp));
+    const int ch = part_keys(len, A.ns), lo = part * ch, hi = min(len, lo + ch);
+    if (lo >= hi) {
+      // no key: the part's sum says so, or, as the only part, the output is zero
+      const int n = min(16, A.g - 16 * tile) * (D / 4);
+      for (int i = threadIdx.x; i < n; i += 64 * AW)
+        if (A.np + A.ns == 1 || i % (D / 4) == 0)
+          store_o<F16, D>(A, A.np + part, h, b, 16 * tile + i / (D / 4), 4 * (i % (D / 4)), f32x4{0.f, 0.f, 0.f, 0.f}, -INFINITY,
+                          0.f);
+      return;
+    }
+    const Run mine[1] = {{A.tables + (size_t)b * A.t_sb + (size_t)h * A.t_sh, lo, hi}};
+    own_part<F16, D, 1>(A, mine, h, b, 16 * tile, A.g, A.np + part, lds, s_m, s_l);
   }
-  const int tile = id % A.own_tiles;
-  id /= A.own_tiles;
-  const int b = id % A.batch, part = id / A.batch;
-  const int len = max(0, min(A.lens[b] + A.len_add, A.width << A.lp));
-  const int ch = part_keys(len, A.ns), lo = part * ch, hi = min(len, lo + ch);
-  if (lo >= hi) {
-    // no key: the part's sum says so, or, as the only part, the output is zero
-    const int n = min(16, A.g - 16 * tile) * (D / 4);
-    for (int i = threadIdx.x; i < n; i += 64 * AW)
-      if (A.np + A.ns == 1 || i % (D / 4) == 0)
-        store_o<F16, D>(A, A.np + part, h, b, 16 * tile + i / (D / 4), 4 * (i % (D / 4)), f32x4{0.f, 0.f, 0.f, 0.f}, -INFINITY, 0.f);
-    return;
-  }
-  own_part<F16, D, 1>(A, A.tables + (size_t)b * A.t_sb + (size_t)h * A.t_sh, h, b, 16 * tile, A.g, lo, hi, A.np + part, lds, s_m,
-                      s_l);
 }
 
 // A wave a row (query head, sequence): the parts' outputs, scaled to their common maximum, over their sums.
@@ -1011,12 +1037,23 @@ int append_rows(const AppendArgs& A, bool f16, hipStream_t stream) {
 // ones 42.0 us with 512 workgroups for the prefix, 34.4 with 256, 29.6 with 128; 256 behind 15001 with up to
 // 1024 144, 127, 127; without own rows 52.6, 57.5, 90.9 for 16384). Its time is taken as 1.45 us for 64 keys
 // of a tile, one workgroup a CU, the own rows' as their bytes, half of the longest a sequence, at 5.4 TB/s.
+//
+// Short contexts of few sequences take one launch instead (JOINED), whose workgroups go over prefix and own rows alike:
+// up to 640 keys the two cost the GPU the same (4 sequences behind 512 rows 7.3 us in two launches, 7.6 in one; 32
+// sequences 9.3 and 9.1), past them one workgroup's walk is the longer one (1000 keys 8.1 and 12.7), and a
+// launch costs the host 3 us (that call 17.4 us, 14.1 in one launch).
+constexpr int JOINED_KEYS = 640;
 AttnPlan plan_attention(int batch, int hkv, int g, int d, int prefix_len, int max_len) {
   AttnPlan p{};
   constexpr int WANT = 512;
   const int rows = batch * g;
-  p.form = rows <= 16 ? ROWS16 : rows <= 32 ? ROWS32 : rows <= 64 ? ROWS64 : ROWS128;
   p.own_tiles = (g + 15) / 16;
+  if (prefix_len > 0 && max_len > 0 && prefix_len + max_len <= JOINED_KEYS && (long long)batch * hkv * p.own_tiles <= NUM_CUS) {
+    p.form = JOINED;
+    p.ns = 1;
+    return p;
+  }
+  p.form = rows <= 16 ? ROWS16 : rows <= 32 ? ROWS32 : rows <= 64 ? ROWS64 : ROWS128;
   auto parts = [&](int len, long long tiles, double want) {
     const int most = (len + UNIT - 1) / UNIT;
     double n = ceil(want / (double)tiles);
@@ -1044,6 +1081,7 @@ static void attn_launch(const AttnArgs& A, int form, unsigned blocks, hipStream_
       case ROWS16: attn_kernel<F16, D, ROWS16><<<blocks, 64 * AW, 0, stream>>>(A); break;
       case ROWS32: attn_kernel<F16, D, ROWS32><<<blocks, 64 * AW, 0, stream>>>(A); break;
       case ROWS64: attn_kernel<F16, D, ROWS64><<<blocks, 64 * AW, 0, stream>>>(A); break;
+      case JOINED: attn_kernel<F16, D, JOINED><<<blocks, 64 * AW, 0, stream>>>(A); break;
       default: attn_kernel<F16, D, ROWS128><<<blocks, 64 * AW, 0, stream>>>(A); break;
     }
   }

@@ -262,6 +262,12 @@ SHARED = [
     (1, 8, 2, 128, 16, BF, 0, [9000]),
     (1, 8, 2, 64, 16, FP, 9001, [40]),
     (65, 1, 8, 64, 64, BF, 4000, [i for i in range(65)]),
+    (40, 8, 2, 128, 64, BF, 4000, [(13 * i) % 65 for i in range(40)]),
+    (32, 8, 1, 128, 32, FP, 500, [(29 * i) % 130 for i in range(32)]),
+    (33, 8, 1, 128, 32, FP, 500, [(29 * i) % 130 for i in range(33)]),
+    (6, 2, 2, 64, 16, BF, 601, [39, 0, 20, 1, 38, 16]),
+    (6, 2, 2, 64, 16, BF, 609, [39, 0, 20, 1, 38, 16]),
+    (130, 2, 1, 128, 64, BF, 200, [0] * 130),
 ]
 
 
