@@ -190,8 +190,9 @@ __global__ void __launch_bounds__(CT) append_kernel(AppendArgs A) {
 // Scores come transposed, S^T = K Q^T: a lane holds 4 keys of each 16-key tile for one query row, so
 // the softmax needs one reduction over the four lane groups, and its probabilities are already the
 // operand of O^T = V^T P^T, whose V^T comes from LDS by transpose reads in the same key order. The
-// probabilities are rounded to 16 bits for that product (a relative 2^-9 (bf16) of each term, as
-// much as the output's own rounding); maxima, sums and outputs stay in 32 bits.
+// probabilities are rounded to the type for that product (at most a relative 2^-8 of a term in bf16, 2^-11
+// in fp16, as much as the output's own rounding; the sum they are divided by is that of the rounded
+// ones); maxima, sums and outputs stay in 32 bits.
 constexpr int NUM_CUS = 256;
 constexpr int AW = 4;   // waves
 constexpr int KS = 32;  // keys a wave takes at a time, of own rows
@@ -613,6 +614,12 @@ __device__ __forceinline__ void prefix_part(const AttnArgs& A, int h, int row0, 
   }
 }
 
+// positions that a sequence has: lens[b] and what was appended since, within its table
+__device__ __forceinline__ int own_rows(const int* lens, int b, int add, int width, int lp) {
+  const int most = width << lp;
+  return max(0, min(min(lens[b], most) + add, most));
+}
+
 // keys of one part of `parts` of `len` keys, in units of 128 (a step for each wave, two of the prefix)
 constexpr int UNIT = KS * AW;
 __host__ __device__ __forceinline__ int part_keys(int len, int parts) { return ((len + parts - 1) / parts + UNIT - 1) / UNIT * UNIT; }
@@ -631,7 +638,7 @@ __global__ void __launch_bounds__(64 * AW, 2) attn_kernel(AttnArgs A) {
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&s_kv[0];
   if constexpr (FORM == JOINED) {
     const int h = blockIdx.x % A.hkv, id = blockIdx.x / A.hkv, tile = id % A.own_tiles, b = id / A.own_tiles;
-    const int len = max(0, min(A.lens[b] + A.len_add, A.width << A.lp));
+    const int len = own_rows(A.lens, b, A.len_add, A.width, A.lp);
     const Run runs[2] = {{A.prefix_pages, 0, A.prefix_len}, {A.tables + (size_t)b * A.t_sb + (size_t)h * A.t_sh, 0, len}};
     own_part<F16, D, 1>(A, runs, h, b, 16 * tile, A.g, 0, lds, s_m, s_l);
   } else {
@@ -656,7 +663,7 @@ __global__ void __launch_bounds__(64 * AW, 2) attn_kernel(AttnArgs A) {
     const int tile = id % A.own_tiles;
     id /= A.own_tiles;
     const int b = id % A.batch, part = id / A.batch;
-    const int len = max(0, min(A.lens[b] + A.len_add, A.width << A.lp));
+    const int len = own_rows(A.lens, b, A.len_add, A.width, A.lp);
     const int ch = part_keys(len, A.ns), lo = part * ch, hi = min(len, lo + ch);
     if (lo >= hi) {
       // no key: the part's sum says so, or, as the only part, the output is zero
@@ -807,7 +814,7 @@ __global__ void __launch_bounds__(ST) select_kernel(SelectArgs A) {
   __shared__ uint32_t s_cnt[2][ST / 64];
   __shared__ int s_id[ST];  // (of up to ST pages)
   const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-  const int len = max(0, min(A.lens[b] + A.len_add, A.width << A.lp)), used = (len + (1 << A.lp) - 1) >> A.lp;
+  const int len = own_rows(A.lens, b, A.len_add, A.width, A.lp), used = (len + (1 << A.lp) - 1) >> A.lp;
   const int* table = A.tables + (size_t)b * A.t_sb;
   int* chosen = A.chosen + ((size_t)b * A.hkv + h) * A.top;
   int* pages = A.pages + ((size_t)b * A.hkv + h) * A.top;
@@ -970,6 +977,7 @@ static bool ids_ok(const int* ids, int n, int num_pages) {
     if (ids[i] < 0 || ids[i] >= num_pages) return false;
   return true;
 }
+constexpr int MAX_KEYS = 1 << 30;  // (sums of lengths stay in 32 bits)
 static int log2_of(int x) { return __builtin_ctz((unsigned)x); }
 
 template <int N>
@@ -1131,7 +1139,7 @@ int shared_attention(const MqPagePool* P, const void* q, int64_t q_sb, int64_t q
                      int width, const int* lens, int len_add, int max_len, float scale, void* ws, size_t ws_bytes,
                      hipStream_t stream) {
   if (!attn_ok(P, false, q, q_sb, q_sh, out, o_sb, o_sh, num_q_heads, batch, tables, t_sb, width, lens, scale, ws) ||
-      prefix_len < 0 || (prefix_len > 0 && !prefix_pages) || max_len < 0)
+      prefix_len < 0 || prefix_len > MAX_KEYS || (prefix_len > 0 && !prefix_pages) || max_len < 0 || max_len > MAX_KEYS)
     return MQ_ERR_ARG;
   const AttnPlan p = plan_attention(batch, P->num_kv_heads, num_q_heads / P->num_kv_heads, P->head_dim, prefix_len, max_len);
   if (ws_bytes < p.bytes) return MQ_ERR_ARG;
@@ -1226,7 +1234,7 @@ extern "C" int mq_pages_append(const MqPagePool* pool, const void* k, const void
 extern "C" int mq_attention_workspace(const MqPagePool* pool, int num_q_heads, int batch, int prefix_len, int max_len, int top,
                                       size_t* bytes) {
   if (!pool || !bytes || pool->num_kv_heads < 1 || num_q_heads < pool->num_kv_heads || num_q_heads % pool->num_kv_heads ||
-      batch < 1 || prefix_len < 0 || max_len < 0 || top < 0)
+      batch < 1 || prefix_len < 0 || prefix_len > MAX_KEYS || max_len < 0 || max_len > MAX_KEYS || top < 0)
     return MQ_ERR_ARG;
   *bytes = plan_attention(batch, pool->num_kv_heads, num_q_heads / pool->num_kv_heads, pool->head_dim, prefix_len, max_len).bytes +
            (top > 0 ? chosen_bytes(batch, pool->num_kv_heads, top) : 0);

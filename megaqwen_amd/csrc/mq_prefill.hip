@@ -2268,7 +2268,7 @@ static BatchBufs batch_bufs(int batch, int prefix_len, int max_len, int top, int
 static bool batch_args_ok(const MqPagePool* P, int batch, int prefix_len, int max_len, int top, int width) {
   return P && P->num_kv_heads == NKV && P->head_dim == HD && P->dtype == MQ_BF16 && P->num_layers >= 1 &&
          P->num_layers <= MAX_LAYERS && P->page_size >= 16 && P->page_size <= 256 && (P->page_size & (P->page_size - 1)) == 0 &&
-         batch >= 1 && batch <= MAX_BATCH && prefix_len >= 0 && max_len >= 1 && top >= 0 && top <= MQ_MAX_TABLE_WIDTH &&
+         batch >= 1 && batch <= MAX_BATCH && prefix_len >= 0 && prefix_len <= 1 << 30 && max_len >= 1 && max_len <= 1 << 30 && top >= 0 && top <= MQ_MAX_TABLE_WIDTH &&
          (top == 0 || (prefix_len == 0 && P->bounds)) && width >= 1 && width <= MQ_MAX_TABLE_WIDTH;
 }
 

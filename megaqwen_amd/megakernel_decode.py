@@ -512,9 +512,9 @@ class MegakernelBatchDecoder:
                     self.sparse_pages_, d.attn_scale_, _ptr(ws), size.value)
         got = out.tolist()
         cache.extend([s for s, t in zip(seqs, got) if t >= 0])
+        self._key = (tuple(seqs), cache.version)  # (the launch has advanced the lengths on the GPU likewise)
         bad = {s: -t - 1 for s, t in zip(seqs, got) if t < 0}
         if bad:
-            self._key = None
             raise _abi.MegakernelError(f"batch step failed for sequences {bad} (flags: 1 token id, 2 position, 4 page); "
                                        f"their lengths are unchanged")
         return got, logits
@@ -867,6 +867,8 @@ class MegakernelPrefillGenerator(_GeneratorBase):
         shared. Without do_sample all n are the greedy one. sparse_pages: see MegakernelBatchDecoder."""
         if not 1 <= n <= 1024:
             raise ValueError("n must be in [1, 1024]")
+        if sparse_pages is not None and sparse_pages < 1:
+            raise ValueError("sparse_pages must be positive")
         g = self._sampling(do_sample, temperature, seed)
         ids = self._ids(prompt)
         if not ids:

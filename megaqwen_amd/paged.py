@@ -288,7 +288,7 @@ class PagedKVCache:
         self._users = [0] * num_pages
         self._seqs: dict[int, list] = {}  # sequence -> [pages, rows]
         self._next = 0
-        self.version = 0  # changes with every change of a page list
+        self.version = 0  # changes with every change of a page list or a length
 
     # -- the books ---------------------------------------------------------------
     def _of(self, seq: int) -> list:
@@ -327,10 +327,12 @@ class PagedKVCache:
         return seq
 
     def fork(self, seq: int, n: int = 1) -> list[int]:
-        """n sequences with the rows of `seq`, whose pages they share. No row is copied."""
+        """n sequences with the rows of `seq`, whose pages they share. No row is copied. (Pages that were reserved
+        and hold no row yet stay `seq`'s alone.)"""
         pages, rows = self._of(seq)
         if n < 0:
             raise ValueError("n must not be negative")
+        pages = pages[: -(-rows // self.page_size)]
         out = []
         for _ in range(n):
             s = self.new()
@@ -392,6 +394,7 @@ class PagedKVCache:
                 raise ValueError(f"sequence {s}: {n} + {rows} rows do not fit its {len(pages)} pages")
         for s in seqs:
             self._seqs[s][1] += rows
+        self.version += 1
 
     def load(self, seq: int, k_cache, v_cache, length: int) -> None:
         """Rows 0 .. length - 1 of contiguous caches as all of the sequence's rows (it has none yet)."""

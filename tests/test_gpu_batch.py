@@ -154,6 +154,31 @@ def test_sparse_pages(small):
     assert bool(results[2].isfinite().all()) and not torch.equal(results[0], results[2])
 
 
+def test_rows_that_a_user_appends_between_steps(small):
+    """The pool is the user's too: rows appended with append_rows and extend count in the next step of the same sequences."""
+    dec, _ = small
+    prompt = weights.random_prompt(100, seed=30)
+    b = MK.MegakernelBatchDecoder(dec, max_batch=2, page_size=64, num_pages=20)
+    seq, _ = b.prefill(prompt)
+    one, two = b.fork(seq, 2)
+    cache = b.cache
+    b.step([one], [1])
+    b.step([two], [1])
+    cache.reserve([one])
+    tables, lens = cache.tables([one])
+    row = torch.randn(2, 1, 8, 128, device="cuda").to(torch.bfloat16)
+    for l in range(2):
+        paged.append_rows(row[l], row[l], cache.k_pages[l], cache.v_pages[l], tables, lens)
+    cache.extend([one])
+    got = b.step_with_logits([one], [7])[1]
+    # the same rows by way of the batch-1 cache
+    dec.reset()
+    b.to_decoder(two)
+    dec.k_cache_[:, :, 101], dec.v_cache_[:, :, 101] = row[:, 0], row[:, 0]
+    dec.set_position(102)
+    _close(got[0], dec.decode_step_with_logits(7)[1])
+
+
 def test_step_refusals(small):
     dec, _ = small
     b = MK.MegakernelBatchDecoder(dec, max_batch=2, page_size=16, num_pages=3)

@@ -85,7 +85,7 @@ COMMON = [dict(q=None), dict(q=8), dict(out=None), dict(out=24), dict(q_sb=4), d
           dict(ws=None), dict(ws=8)]
 
 
-@pytest.mark.parametrize("bad", COMMON + [dict(prefix_len=-1), dict(prefix_pages=None), dict(max_len=-1), dict(prefix_len=2000, ws_bytes=16)], ids=str)
+@pytest.mark.parametrize("bad", COMMON + [dict(prefix_len=-1), dict(prefix_len=2 ** 30 + 1), dict(prefix_pages=None), dict(max_len=-1), dict(max_len=2 ** 31 - 1), dict(prefix_len=2000, ws_bytes=16)], ids=str)
 def test_shared_prefix_attention_refuses(bad):
     assert _shared(**bad) == _abi.MQ_ERR_ARG
 
@@ -363,6 +363,46 @@ def test_fork_copies_a_page_only_when_it_is_written(cpu_pages):
     cache.free(a)
     cache.free(b)
     assert _rows(cache, c)[-1] == 102.0 and cache.free_pages() == 38
+
+
+def test_a_fork_leaves_reserved_pages_behind(cpu_pages):
+    """Pages that hold no row yet are not shared: two sequences that go on from there write to pages of their own."""
+    cache = _cache()
+    a = cache.new()
+    for i in range(16):
+        _grow(cache, [a], [float(i)])
+    cache.reserve([a], 20)  # pages for positions 16 .. 35
+    assert len(cache.pages(a)) == 3
+    b = cache.fork(a)[0]
+    assert cache.pages(b) == cache.pages(a)[:1]
+    _check_books(cache)
+    _grow(cache, [a, b], [50.0, 60.0])
+    assert cache.pages(a)[1] != cache.pages(b)[1]
+    assert _rows(cache, a)[-1] == 50.0 and _rows(cache, b)[-1] == 60.0
+
+
+def test_every_change_changes_the_version(cpu_pages):
+    cache = _cache()
+    seen = [cache.version]
+
+    def changed():
+        seen.append(cache.version)
+        return seen[-1] != seen[-2]
+
+    a = cache.new()
+    cache.reserve([a], 3)
+    assert changed()
+    cache.extend([a], 3)
+    assert changed()
+    b = cache.fork(a)[0]
+    cache.reserve([a], 1)
+    assert changed()  # (a page of its own)
+    cache.free(a)
+    assert changed()
+    cache.compact()
+    kc = torch.zeros(1, 1, 40, 64, dtype=BF)
+    cache.load(cache.new(), kc, kc, 7)
+    assert changed() and cache.length(b) == 3
 
 
 def test_a_full_shared_page_is_not_copied(cpu_pages):
