@@ -297,21 +297,23 @@ __device__ __forceinline__ uint32_t v_frag(int r16, int kg) {
   return row * (2 * D) + 16 * (((r16 & 3) >> 1) ^ swz<D>(row)) + 8 * (r16 & 1);
 }
 
-// m is the maximum that a row's probabilities are taken relative to; it follows the true one once that is
-// 2^SLACK times as large as it, so that few steps have to rescale l and o (their 64 products a 64-key step were
-// 40% of all vector instructions: with each new maximum of any of 16 rows, 51 us for the prefix of 15001
-// rows and 512 queries). Probabilities reach 2^SLACK then, which no type here minds.
-constexpr float SLACK = 8.f;
+// m is the maximum that a row's probabilities are taken relative to. Where the matrix units are the bound
+// (prefix_part) it follows the true one only once that is 2^SLACK times as large, so that few steps have to rescale l
+// and o (64 products a 64-key step, 40% of all vector instructions there; the prefix of 16384 rows for 512 query rows
+// 61.0 us at 0, 58.8 at 1, 57.8 at 8). Where memory is (own_part) it is the maximum. The nearer it is, the less
+// the heaviest terms, just below 1 then, round: bf16 outputs are a relative 2.3e-3 from the 64-bit ones at 8, 2.1e-3 at 0
+// (the output's own rounding alone: 1.7e-3).
+constexpr float SLACK = 1.f;
 
 // One step of NT key tiles (K and V rows in LDS at kb and vb) for RB * 16 query rows: running maximum m of
 // query row r16 of each block, sum l (four equal values) and output o (lane: dims 16 dt + 4 kg + e of row r16).
 // `left`: keys of the step that are there. before_v() runs between the scores and the product with V.
-// The vector units are the tighter bound here (two products a score pair cost the matrix units 1024 cycles a
-// 64-key step of 32 rows), so the sum of the probabilities is another row of the product, with ones
+// The vector units are the tighter bound here (the products of a 64-key step of 32 rows cost the matrix units 1024
+// cycles), so the sum of the probabilities is another row of the product, with ones
 // for V, and the maximum takes three operands (v_maximum3_f32; a score that is not a number
 // makes its row's output not a number either way).
 template <bool F16, int D, int RB, int NT, class BeforeV>
-__device__ __forceinline__ void attend_step(uint32_t kb, uint32_t vb, int left, float scale, int kg, uint32_t ka, uint32_t va,
+__device__ __forceinline__ void attend_step(uint32_t kb, uint32_t vb, int left, float scale, float slack, int kg, uint32_t ka, uint32_t va,
                                             const u32x4 (&qf)[RB][D / 32], float (&m)[RB], f32x4 (&l)[RB],
                                             f32x4 (&o)[RB][D / 16], BeforeV before_v) {
   f32x4 sc[RB][NT];
@@ -357,7 +359,7 @@ __device__ __forceinline__ void attend_step(uint32_t kb, uint32_t vb, int left, 
     for (int t = 0; t < NT; t++)
       mx[rb] = max3(max3(mx[rb], sc[rb][t][0], sc[rb][t][1]), sc[rb][t][2], sc[rb][t][3]);
     mx[rb] = fmaxf(m[rb], groups_max(mx[rb]) * scale);
-    raise |= mx[rb] > m[rb] + SLACK;
+    raise |= mx[rb] > m[rb] + slack;
   }
   if (__any(raise)) {
 #pragma unroll
@@ -504,7 +506,7 @@ __device__ __forceinline__ void own_part(const AttnArgs& A, const Run (&runs)[N]
     for (; k0 < k_hi; k0 += KS * AW) {
       const int next = k0 + KS * AW;
       PG_AWAIT(NI);  // K is there (V may be in flight)
-      attend_step<F16, D, RB, KS / 16>(mine, mine + HALF, k_hi - k0, A.scale_log2, kg, ka, va, qf, m, l, o, [&] {
+      attend_step<F16, D, RB, KS / 16>(mine, mine + HALF, k_hi - k0, A.scale_log2, 0.f, kg, ka, va, qf, m, l, o, [&] {
         PG_READ();  // (K is in registers)
         if (next < k_hi) {
           find(next);
@@ -600,7 +602,7 @@ __device__ __forceinline__ void prefix_part(const AttnArgs& A, int h, int row0, 
   for (int k0 = k_lo; k0 < k_hi; k0 += TS, st ^= STAGE) {
     PG_BARRIER();
     if (k0 + TS < k_hi) fetch(k0 + TS, lds + (st ^ STAGE));
-    attend_step<F16, D, RB, TS / 16>(lds + st, lds + st + HALF, k_hi - k0, A.scale_log2, kg, ka, va, qf, m, l, o, [] {});
+    attend_step<F16, D, RB, TS / 16>(lds + st, lds + st + HALF, k_hi - k0, A.scale_log2, SLACK, kg, ka, va, qf, m, l, o, [] {});
   }
   // every wave has seen some of the page ids: a bad one anywhere reaches all rows of the tile
   const int bad = __syncthreads_or(pages.bad);
