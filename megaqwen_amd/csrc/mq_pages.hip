@@ -238,10 +238,14 @@ typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
 typedef __attribute__((address_space(3))) uint8_t lds_byte;
 typedef const __attribute__((address_space(1))) int gint;
 
-// the swizzle of a row's 16-byte pieces (D / 8 of them): 256-byte rows all start at the same bank,
-// 128-byte ones in pairs
+// The swizzle of a row's 16-byte pieces (D / 8 of them), by XOR with the piece's number: the rows that one read
+// takes together fall in distinct banks. 256-byte rows all start at the same bank, 128-byte ones in pairs. K is
+// read 16 rows of a piece at a time, V by transpose reads, 8 rows of two neighbouring pieces at a time. No read
+// of either meets another one's bank (counted: SQ_LDS_BANK_CONFLICT 0).
 template <int D>
-__device__ __forceinline__ int swz(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
+__device__ __forceinline__ int swz_k(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
+template <int D>
+__device__ __forceinline__ int swz_v(int row) { return D == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 3); }
 
 // A value that a plain load brought, used here: the compiler, which does not count the DMA instructions, waits
 // for it at this place, and not (for every load and DMA under way) at its next use inside a loop
@@ -272,29 +276,68 @@ struct Pages {
   }
 };
 
-// 16 consecutive keys from k0 (a multiple of 16, so of one page) of K or V, to LDS: NI DMA
-// instructions. Rows past k_last repeat it, from its page `clamp` (their scores are masked, and a
-// row that is not there is never read).
-template <int D, bool ONCE>
-__device__ __forceinline__ void fetch16(const uint16_t* pool, size_t base, int k0, int k_last, int pmask, uint32_t dst, int lane) {
-  constexpr int CPR = D / 8, RPI = 64 / CPR, NI = 16 / RPI;  // pieces a row, rows an instruction
-#pragma unroll
-  for (int i = 0; i < NI; i++) {
-    const int row = RPI * i + lane / CPR, key = min(k0 + row, k_last);
-    const uint16_t* src = pool + base + (size_t)((key & pmask) * D + 8 * ((lane % CPR) ^ swz<D>(row)));
-    const uint32_t to = __builtin_amdgcn_readfirstlane(dst + 1024u * i);
-    if (ONCE) dma16_nt(src, to); else dma16(src, to);
-  }
+// One DMA instruction: lane l's 16 bytes at base + off to LDS byte lds + 16 l (dma16 with a uniform base, so that a
+// step's addresses cost no vector instruction; ONCE: past the caches)
+template <bool ONCE>
+__device__ __forceinline__ void dma16_at(const uint16_t* base, uint32_t off, uint32_t lds) {
+  uint32_t saved;
+  if constexpr (ONCE)
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dwordx4 %1, %2 nt\n\ts_mov_b32 m0, %0"
+                 : "=&s"(saved)
+                 : "v"(off), "s"(base), "s"(lds)
+                 : "memory");
+  else
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+                 : "=&s"(saved)
+                 : "v"(off), "s"(base), "s"(lds)
+                 : "memory");
 }
+
+// Byte offsets, from a 16-key tile's first row, of the pieces that a lane brings: instruction i moves rows RPI i ..,
+// lane l -> row RPI i + l / CPR, slot l % CPR, which takes the piece that the swizzle puts there
+template <int D, bool V>
+struct Lanes {
+  static constexpr int CPR = D / 8, RPI = 64 / CPR, NI = 16 / RPI;  // pieces a row, rows an instruction, instructions
+  uint32_t off[NI];
+  __device__ __forceinline__ explicit Lanes(int lane) {
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+      const int row = RPI * i + lane / CPR;
+      off[i] = row * (2 * D) + 16 * ((lane % CPR) ^ (V ? swz_v<D>(row) : swz_k<D>(row)));
+    }
+  }
+  // the tile at `base` to LDS; rows past `last` repeat it (their scores are masked; a row that is not there is never read)
+  template <bool ONCE>
+  __device__ __forceinline__ void fetch(const uint16_t* base, int last, uint32_t dst, int lane) const {
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+      uint32_t o = off[i];
+      if (last < 15) o -= max(0, RPI * i + lane / CPR - last) * (2 * D);
+      dma16_at<ONCE>(base, o, __builtin_amdgcn_readfirstlane(dst + 1024u * i));
+    }
+  }
+};
+
+// Where the 16-key tile at key k0 (or, past the last key, that key's tile) lies in a layer's K (and V), and the last
+// row of it that is there
+struct Tile {
+  size_t at;
+  int last;
+  __device__ __forceinline__ Tile(Pages& pages, const AttnArgs& A, int h, int d, int k0, int k_last, int lane) {
+    const int k = min(k0, k_last & ~15);
+    at = (((((size_t)pages(k >> A.lp, lane) * A.hkv + h) << A.lp) + (k & ((1 << A.lp) - 1))) * d);
+    last = k_last - k;
+  }
+};
 
 // Fragment addresses in 16-key tiles of LDS rows: K row r16, pieces 4 ks + kg; V keys 4 kg + r16 / 4, dims
 // 16 dt + 4 (r16 % 4) .. + 3 (a tile t adds 32 t D bytes; ks and dt come in by XOR)
 template <int D>
-__device__ __forceinline__ uint32_t k_frag(int r16, int kg) { return r16 * (2 * D) + 16 * (kg ^ swz<D>(r16)); }
+__device__ __forceinline__ uint32_t k_frag(int r16, int kg) { return r16 * (2 * D) + 16 * (kg ^ swz_k<D>(r16)); }
 template <int D>
 __device__ __forceinline__ uint32_t v_frag(int r16, int kg) {
   const int row = 4 * kg + (r16 >> 2);
-  return row * (2 * D) + 16 * (((r16 & 3) >> 1) ^ swz<D>(row)) + 8 * (r16 & 1);
+  return row * (2 * D) + 16 * (((r16 & 3) >> 1) ^ swz_v<D>(row)) + 8 * (r16 & 1);
 }
 
 // m is the maximum that a row's probabilities are taken relative to. Where the matrix units are the bound
@@ -467,9 +510,9 @@ __device__ __forceinline__ void own_part(const AttnArgs& A, const Run (&runs)[N]
   constexpr int NI = KS * D * 2 / 1024;                   // DMA instructions of a step's K (or V)
   static_assert(RB * 16 * D * 4 <= (int)WAVE, "a wave's output fits its LDS");
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, kg = lane >> 4;
-  const int pmask = (1 << A.lp) - 1;
-  const size_t page_elems = ((size_t)A.hkv << A.lp) * D, head_elems = ((size_t)h << A.lp) * D;
   const uint32_t mine = lds + WAVE * wv;
+  const Lanes<D, false> lk(lane);
+  const Lanes<D, true> lv(lane);
   u32x4 qf[RB][D / 32];
   float m[RB];
   f32x4 l[RB], o[RB][D / 16];
@@ -488,19 +531,28 @@ __device__ __forceinline__ void own_part(const AttnArgs& A, const Run (&runs)[N]
     int k0 = runs[n].lo + KS * wv;
     const bool any = k0 < k_hi;  // (the wave's)
     Pages pages(runs[n].table, A.num_pages, runs[n].lo >> A.lp, max(runs[n].lo, k_hi - 1) >> A.lp, lane, any);
-    size_t base[2];  // the pages of a step's two 16-key halves
+    size_t at[2];  // a step's two tiles
+    int last[2];
     auto find = [&](int k0) {
-      base[0] = (size_t)pages(k0 >> A.lp, lane) * page_elems + head_elems;
-      base[1] = A.lp == 4 && k0 + 16 < k_hi ? (size_t)pages((k0 >> 4) + 1, lane) * page_elems + head_elems : base[0];
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const Tile t(pages, A, h, D, k0 + 16 * i, k_hi - 1, lane);
+        at[i] = t.at;
+        last[i] = t.last;
+      }
     };
-    auto fetch = [&](const uint16_t* pool, int k0, uint32_t dst) {
-      fetch16<D, true>(pool, base[0], k0, k_hi - 1, pmask, dst, lane);
-      fetch16<D, true>(pool, base[1], k0 + 16, k_hi - 1, pmask, dst + HALF / 2, lane);
+    auto fetch_k = [&] {
+#pragma unroll
+      for (int i = 0; i < 2; i++) lk.template fetch<true>(A.k + at[i], last[i], mine + HALF / 2 * i, lane);
+    };
+    auto fetch_v = [&] {
+#pragma unroll
+      for (int i = 0; i < 2; i++) lv.template fetch<true>(A.v + at[i], last[i], mine + HALF + HALF / 2 * i, lane);
     };
     if (any) {
       find(k0);
-      fetch(A.k, k0, mine);
-      fetch(A.v, k0, mine + HALF);
+      fetch_k();
+      fetch_v();
     }
     if (n == 0) load_q<D, RB>(A, h, b0, row0, rows, r16, kg, qf);
     for (; k0 < k_hi; k0 += KS * AW) {
@@ -510,14 +562,14 @@ __device__ __forceinline__ void own_part(const AttnArgs& A, const Run (&runs)[N]
         PG_READ();  // (K is in registers)
         if (next < k_hi) {
           find(next);
-          fetch(A.k, next, mine);
+          fetch_k();
           PG_AWAIT(NI);  // V is there (the next K may be in flight)
         } else {
           PG_AWAIT(0);
         }
       });
       PG_READ();
-      if (next < k_hi) fetch(A.v, next, mine + HALF);
+      if (next < k_hi) fetch_v();
     }
     bad |= pages.bad;
   }
@@ -569,20 +621,23 @@ __device__ __forceinline__ void own_part(const AttnArgs& A, const Run (&runs)[N]
 // Keys [k_lo, k_hi) of the prefix for up to 64 RB query rows from row0 of all `rows`: wave w takes RB blocks
 // of 16 rows from row0 + 16 RB w and all the keys, 64 at a time, from LDS that the workgroup fills together
 // (two stages: the next one is on its way while this one is multiplied). One barrier a step: once every
-// wave is there, the stage is complete and the other one has been read.
+// wave is there, the stage is complete and the other one has been read. Bound by the vector and matrix units: a
+// step of 32 rows costs a wave 1088 cycles of products and about as many of exponentials (32 at a quarter of the
+// rate) and the rest, and two waves share a SIMD; 16384 rows for 512 query rows keep the matrix units 37% busy.
+// Without any K and V fetched the steps took 1.6 us where they take 2.35; asking for K and V half a step earlier,
+// with a second barrier, or putting the exponentials of one half between the products of the other gained nothing.
 template <bool F16, int D, int RB>
 __device__ __forceinline__ void prefix_part(const AttnArgs& A, int h, int row0, int rows, int k_lo, int k_hi, int slot, uint32_t lds) {
   constexpr uint32_t HALF = TS * D * 2, STAGE = 2 * HALF;
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, kg = lane >> 4;
-  const int pmask = (1 << A.lp) - 1;
-  const size_t page_elems = ((size_t)A.hkv << A.lp) * D, head_elems = ((size_t)h << A.lp) * D;
+  const Lanes<D, false> lk(lane);
+  const Lanes<D, true> lv(lane);
   Pages pages(A.prefix_pages, A.num_pages, k_lo >> A.lp, (k_hi - 1) >> A.lp, lane, true);
-  // wave w brings keys 16 w .. + 15 of a step; a step's first page past the end is its last key's
+  // wave w brings keys 16 w .. + 15 of a step
   auto fetch = [&](int k0, uint32_t dst) {
-    const int k = min(k0 + 16 * wv, k_hi - 1);
-    const size_t base = (size_t)pages(k >> A.lp, lane) * page_elems + head_elems;
-    fetch16<D, false>(A.k, base, k0 + 16 * wv, k_hi - 1, pmask, dst + HALF / 4 * wv, lane);
-    fetch16<D, false>(A.v, base, k0 + 16 * wv, k_hi - 1, pmask, dst + HALF + HALF / 4 * wv, lane);
+    const Tile t(pages, A, h, D, k0 + 16 * wv, k_hi - 1, lane);
+    lk.template fetch<false>(A.k + t.at, t.last, dst + HALF / 4 * wv, lane);
+    lv.template fetch<false>(A.v + t.at, t.last, dst + HALF + HALF / 4 * wv, lane);
   };
   fetch(k_lo, lds);
   u32x4 qf[RB][D / 32];
