@@ -303,7 +303,7 @@ int mq_pages_append(const MqPagePool* pool, const void* k, const void* v, long l
                     const int* lens, int batch, hipStream_t stream);
 
 /* Bytes of workspace of one call of the attentions below: prefix_len, max_len and num_q_heads as
- * given to it; top 0 for mq_shared_prefix_attention. For mq_sparse_attention prefix_len is 0 and
+ * given to it (0: the call takes NULL); top 0 for mq_shared_prefix_attention. For mq_sparse_attention prefix_len is 0 and
  * max_len min(top, width) * page_size. */
 int mq_attention_workspace(const MqPagePool* pool, int num_q_heads, int batch, int prefix_len, int max_len, int top,
                            size_t* bytes);

@@ -1168,15 +1168,18 @@ int run_attention(AttnArgs A, const AttnPlan& p, int d, bool f16, void* ws, hipS
   return hipGetLastError() == hipSuccess ? MQ_OK : MQ_ERR_HIP;
 }
 
+// (a call that needs none takes NULL)
+static bool workspace_ok(const void* ws, size_t has, size_t needs) { return needs == 0 || (ws && aligned16(ws) && has >= needs); }
+
 static bool rows_ok(const void* p, int64_t sb, int64_t sh) { return p && aligned16(p) && sb % 8 == 0 && sh % 8 == 0; }
 
 // What both attentions ask of their common arguments.
 static bool attn_ok(const MqPagePool* P, bool sparse, const void* q, int64_t q_sb, int64_t q_sh, const void* out, int64_t o_sb,
                     int64_t o_sh, int num_q_heads, int batch, const int* tables, int64_t t_sb, int width, const int* lens,
-                    float scale, const void* ws) {
+                    float scale) {
   return pool_ok(P, sparse) && rows_ok(q, q_sb, q_sh) && rows_ok(out, o_sb, o_sh) && batch >= 1 && batch <= 65535 &&
          num_q_heads >= P->num_kv_heads && num_q_heads <= 16384 && num_q_heads % P->num_kv_heads == 0 && tables && lens &&
-         width >= 1 && width <= MQ_MAX_TABLE_WIDTH && t_sb >= 0 && scale > 0.f && isfinite(scale) && ws && aligned16(ws);
+         width >= 1 && width <= MQ_MAX_TABLE_WIDTH && t_sb >= 0 && scale > 0.f && isfinite(scale);
 }
 
 static AttnArgs attn_args(const MqPagePool& P, const void* q, int64_t q_sb, int64_t q_sh, void* out, int64_t o_sb,
@@ -1195,11 +1198,11 @@ int shared_attention(const MqPagePool* P, const void* q, int64_t q_sb, int64_t q
                      int num_q_heads, int batch, const int* prefix_pages, int prefix_len, const int* tables, int64_t t_sb,
                      int width, const int* lens, int len_add, int max_len, float scale, void* ws, size_t ws_bytes,
                      hipStream_t stream) {
-  if (!attn_ok(P, false, q, q_sb, q_sh, out, o_sb, o_sh, num_q_heads, batch, tables, t_sb, width, lens, scale, ws) ||
+  if (!attn_ok(P, false, q, q_sb, q_sh, out, o_sb, o_sh, num_q_heads, batch, tables, t_sb, width, lens, scale) ||
       prefix_len < 0 || prefix_len > MAX_KEYS || (prefix_len > 0 && !prefix_pages) || max_len < 0 || max_len > MAX_KEYS)
     return MQ_ERR_ARG;
   const AttnPlan p = plan_attention(batch, P->num_kv_heads, num_q_heads / P->num_kv_heads, P->head_dim, prefix_len, max_len);
-  if (ws_bytes < p.bytes) return MQ_ERR_ARG;
+  if (!workspace_ok(ws, ws_bytes, p.bytes)) return MQ_ERR_ARG;
   AttnArgs A = attn_args(*P, q, q_sb, q_sh, out, o_sb, o_sh, num_q_heads, batch, scale);
   A.prefix_pages = prefix_pages; A.prefix_len = prefix_len;
   A.tables = tables; A.t_sb = t_sb; A.width = width; A.lens = lens; A.len_add = len_add;
@@ -1216,13 +1219,13 @@ size_t sparse_workspace(int batch, int hkv, int g, int d, int top, int width, in
 int sparse_attention(const MqPagePool* P, const void* q, int64_t q_sb, int64_t q_sh, void* out, int64_t o_sb, int64_t o_sh,
                      int* chosen, int num_q_heads, int batch, const int* tables, int64_t t_sb, int width, const int* lens,
                      int len_add, int top, float scale, void* ws, size_t ws_bytes, hipStream_t stream) {
-  if (!attn_ok(P, true, q, q_sb, q_sh, out, o_sb, o_sh, num_q_heads, batch, tables, t_sb, width, lens, scale, ws) || !chosen ||
+  if (!attn_ok(P, true, q, q_sb, q_sh, out, o_sb, o_sh, num_q_heads, batch, tables, t_sb, width, lens, scale) || !chosen ||
       top < 1 || top > MQ_MAX_TABLE_WIDTH)
     return MQ_ERR_ARG;
   const int most = top < width ? top : width, hkv = P->num_kv_heads, g = num_q_heads / hkv;
   const AttnPlan p = plan_attention(batch, hkv, g, P->head_dim, 0, most * P->page_size);
   const size_t head = chosen_bytes(batch, hkv, top);
-  if (ws_bytes < head + p.bytes) return MQ_ERR_ARG;
+  if (!workspace_ok(ws, ws_bytes, head + p.bytes)) return MQ_ERR_ARG;
   AttnArgs A = attn_args(*P, q, q_sb, q_sh, out, o_sb, o_sh, num_q_heads, batch, scale);
   SelectArgs S{};
   S.q = A.q; S.bounds = static_cast<const uint16_t*>(P->bounds);

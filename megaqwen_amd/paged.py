@@ -175,7 +175,9 @@ def _query(q, out, pool, like) -> tuple[torch.Tensor, tuple[int, int], tuple[int
     shape = (q.shape[0], q.shape[1], pool.head_dim)
     strides = _rows(q, "q", like, shape)
     if out is None:
-        return torch.empty(shape, dtype=q.dtype, device=q.device), strides, (shape[1] * shape[2], shape[2])
+        out = torch.empty_like(q)
+        sb, sh, _ = out.stride()
+        return out, strides, (sb if shape[0] > 1 else 0, sh if shape[1] > 1 else 0)
     out_strides = _rows(out, "out", like, shape)
     if (shape[0] > 1 and out_strides[0] == 0) or (shape[1] > 1 and out_strides[1] == 0):
         raise ValueError("out: rows that overlap")
@@ -193,7 +195,7 @@ def _scale(scale, head_dim: int) -> float:
 def _workspace_bytes(kv_heads: int, head_dim: int, heads: int, batch: int, prefix_len: int, max_len: int, top: int) -> int:
     n, pool = ctypes.c_size_t(), _abi.MqPagePool(num_kv_heads=kv_heads, head_dim=head_dim)
     _abi.check(_abi.lib().mq_attention_workspace(pool, heads, batch, prefix_len, max_len, top, n), "mq_attention_workspace")
-    return max(n.value, 16)
+    return n.value
 
 
 def shared_prefix_attention(q, k_pages, v_pages, prefix_pages, prefix_len: int, tables, lens, scale: float | None = None,
@@ -225,10 +227,10 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix_pages, prefix_len: int, 
     if max_len < 1:
         raise ValueError("max_len must be positive")
     ws_bytes = _workspace_bytes(pool.num_kv_heads, pool.head_dim, heads, batch, prefix_len, max_len, 0)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
     _call("mq_shared_prefix_attention", k_pages.device, pool, q.data_ptr(), q_sb, q_sh, out.data_ptr(), o_sb, o_sh, heads, batch,
           prefix_pages.data_ptr() if prefix_len else None, prefix_len, tables.data_ptr(), t_sb, width, lens.data_ptr(), max_len,
-          _scale(scale, pool.head_dim), ws.data_ptr(), ws_bytes)
+          _scale(scale, pool.head_dim), ws.data_ptr() if ws_bytes else None, ws_bytes)
     return out
 
 

@@ -308,6 +308,19 @@ def test_shared_prefix_attention_strides_scale_and_out():
     assert torch.equal(_bits(again), _bits(got))
 
 
+def test_query_layouts_that_torch_allows():
+    """Heads before the batch, the same query for all (stride 0), one sequence or one head with a stride that is never used."""
+    from megaqwen_amd import paged
+
+    for B, hkv, G, make in (
+            (5, 2, 3, lambda q: q.transpose(0, 1).contiguous().transpose(0, 1)), (4, 2, 2, lambda q: q[:1].expand(4, -1, -1)),
+            (1, 2, 2, lambda q: q.as_strided(q.shape, (3, q.stride(1), 1))), (3, 1, 1, lambda q: q.as_strided(q.shape, (q.stride(0), 5, 1)))):
+        for prefix in (40, 900):  # (one launch, and two)
+            q, k, v, pre, tables, lens_d, rows_of = _setup(B, hkv, G, 64, 16, BF, prefix, [30 + b for b in range(B)], seed=B)
+            q = make(q)
+            _check(paged.shared_prefix_attention(q, k, v, pre, prefix, tables, lens_d), q, rows_of, 1 / 8)
+
+
 def test_attention_of_large_scores_and_one_sided_values():
     """Scores of hundreds (one key takes all) and values of one sign: no overflow, no bias."""
     from megaqwen_amd import paged

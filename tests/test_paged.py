@@ -82,15 +82,16 @@ def test_append_refuses(bad):
 COMMON = [dict(q=None), dict(q=8), dict(out=None), dict(out=24), dict(q_sb=4), dict(q_sh=65), dict(o_sb=1), dict(o_sh=4), dict(heads=0),
           dict(heads=1), dict(heads=3), dict(batch=0), dict(batch=65536), dict(tables=None), dict(lens=None), dict(width=0),
           dict(width=8193), dict(t_sb=-1), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")),
-          dict(ws=None), dict(ws=8)]
+          dict(scale=-0.0)]
 
 
-@pytest.mark.parametrize("bad", COMMON + [dict(prefix_len=-1), dict(prefix_len=2 ** 30 + 1), dict(prefix_pages=None), dict(max_len=-1), dict(max_len=2 ** 31 - 1), dict(prefix_len=2000, ws_bytes=16)], ids=str)
+@pytest.mark.parametrize("bad", COMMON + [dict(prefix_len=-1), dict(prefix_len=2 ** 30 + 1), dict(prefix_pages=None), dict(max_len=-1), dict(max_len=2 ** 31 - 1), dict(prefix_len=2000, ws_bytes=16),
+                                          dict(prefix_len=2000, ws=None), dict(prefix_len=2000, ws=8)], ids=str)
 def test_shared_prefix_attention_refuses(bad):
     assert _shared(**bad) == _abi.MQ_ERR_ARG
 
 
-@pytest.mark.parametrize("bad", COMMON + [dict(chosen=None), dict(top=0), dict(top=8193), dict(ws_bytes=16)], ids=str)
+@pytest.mark.parametrize("bad", COMMON + [dict(chosen=None), dict(top=0), dict(top=8193), dict(ws_bytes=16), dict(ws=None), dict(ws=8)], ids=str)
 def test_sparse_attention_refuses(bad):
     assert _sparse(**bad) == _abi.MQ_ERR_ARG
     assert _sparse(_pool(bounds=None)) == _abi.MQ_ERR_ARG
