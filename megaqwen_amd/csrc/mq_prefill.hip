@@ -15,6 +15,9 @@
 // argmax_final. Prompts of at most 256 tokens run their layers in one launch instead
 // (mq_prefill_short.hip; the same bits). The GEMMs run on v_mfma_f32_16x16x32_bf16 with fp32 accumulation.
 //
+// The decode step of a batch of sequences (mq_decode_batch, at the end) runs the same products with a sequence a row,
+// over the paged cache of mq_pages.hip; the reference has no counterpart.
+//
 // The intermediates, the fp32 partial sums included, live in the caller's scratch
 // buffers (the reference's own argument list), so a launch allocates nothing.
 //

@@ -268,6 +268,8 @@ SHARED = [
     (6, 2, 2, 64, 16, BF, 601, [39, 0, 20, 1, 38, 16]),
     (6, 2, 2, 64, 16, BF, 609, [39, 0, 20, 1, 38, 16]),
     (130, 2, 1, 128, 64, BF, 200, [0] * 130),
+    (70, 2, 2, 128, 32, FP, 900, [(17 * i) % 200 for i in range(70)]),
+    (40, 1, 4, 128, 256, BF, 1500, [(91 * i) % 600 for i in range(40)]),
 ]
 
 
