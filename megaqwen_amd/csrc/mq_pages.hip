@@ -1100,11 +1100,13 @@ int append_rows(const AppendArgs& A, bool f16, hipStream_t stream) {
 // How an attention call is split. Query rows of the prefix go in tiles of up to 128, so that its keys are read
 // as few times as there are tiles; a sequence's own rows are shared by its G query heads a kv head only, in
 // tiles of 16. Keys are split until the launch has about two workgroups a CU, in parts of at least 128 keys.
-// Beside own rows the prefix takes fewer workgroups, so that it ends about when they do: each part's result
-// is another 4 D + 8 bytes a query row written and read (64 sequences behind 8192 shared rows with up to 512 own
-// ones 42.0 us with 512 workgroups for the prefix, 34.4 with 256, 29.6 with 128; 256 behind 15001 with up to
-// 1024 144, 127, 127; without own rows 52.6, 57.5, 90.9 for 16384). Its time is taken as 1.45 us for 64 keys
-// of a tile, one workgroup a CU, the own rows' as their bytes, half of the longest a sequence, at 5.4 TB/s.
+// Each part's result is another 4 D + 8 bytes a query row written and read, so tiles of more than 32 rows take fewer
+// parts where those cost nothing (us a captured call):
+// - beside own rows as many as end about when these do, at 1.8 us for 64 keys of a tile and 5.4 TB/s for half of the
+//   longest own length a sequence (64 sequences behind 8192 rows with up to 2000 own: 60 against 74 with no such limit;
+//   256 behind 15001 with up to 1024: 113 against 138; at 1.45 us, an alone tile's time, 68 and 120);
+// - of a prefix of few steps, at most 16 each, 192 workgroups, since what a part costs before and after its steps is
+//   several of them (64 behind 8192 with up to 200 own: 24 against 28; 20 behind 15000 with up to 500: 22 against 26).
 //
 // Short contexts of few sequences take one launch instead (JOINED), whose workgroups go over prefix and own rows alike:
 // up to 640 keys the two cost the GPU the same (4 sequences behind 512 rows 7.3 us in two launches, 7.6 in one; 32
@@ -1114,6 +1116,7 @@ constexpr int JOINED_KEYS = 640;
 AttnPlan plan_attention(int batch, int hkv, int g, int d, int prefix_len, int max_len) {
   AttnPlan p{};
   constexpr int WANT = 512;
+  constexpr double STEP_US = 1.8, SHORT_WANT = 192., SHORT_STEPS = 16.;
   const int rows = batch * g;
   p.own_tiles = (g + 15) / 16;
   if (prefix_len > 0 && max_len > 0 && prefix_len + max_len <= JOINED_KEYS && (long long)batch * hkv * p.own_tiles <= NUM_CUS) {
@@ -1131,9 +1134,14 @@ AttnPlan plan_attention(int batch, int hkv, int g, int d, int prefix_len, int ma
   };
   if (prefix_len > 0) {
     p.prefix_tiles = (rows + tile_rows(p.form) - 1) / tile_rows(p.form);
-    const double tiles = (double)hkv * p.prefix_tiles;
-    const double us = tiles * ((prefix_len + TS - 1) / TS) * 1.45, own_us = (double)batch * hkv * max_len * d * 2 / 5.4e6;
-    p.np = parts(prefix_len, (long long)tiles, own_us > 0. ? fmin(us / own_us, WANT) : WANT);
+    const long long tiles = (long long)hkv * p.prefix_tiles;
+    double want = WANT;
+    if (p.form >= ROWS64) {
+      const double steps = (double)tiles * ((prefix_len + TS - 1) / TS), own_us = (double)batch * hkv * max_len * d * 2 / 5.4e6;
+      if (own_us > 0.) want = fmin(want, steps * STEP_US / own_us);
+      if (steps <= SHORT_STEPS * SHORT_WANT) want = fmin(want, SHORT_WANT);
+    }
+    p.np = parts(prefix_len, tiles, want);
   }
   if (max_len > 0) p.ns = parts(max_len, (long long)batch * hkv * p.own_tiles, WANT);
   const size_t rows_all = p.np + p.ns == 1 ? 0 : (size_t)(p.np + p.ns) * batch * hkv * g;
