@@ -302,9 +302,9 @@ int mq_pages_append(const MqPagePool* pool, const void* k, const void* v, long l
                     long long v_sb, long long v_sh, const int* tables, long long table_stride, int width,
                     const int* lens, int batch, hipStream_t stream);
 
-/* Bytes of workspace of one call of the attentions below: prefix_len, max_len and num_q_heads as
- * given to it (0: the call takes NULL); top 0 for mq_shared_prefix_attention. For mq_sparse_attention prefix_len is 0 and
- * max_len min(top, width) * page_size. */
+/* Bytes of workspace of one call of the attentions below (0: the call takes NULL): prefix_len,
+ * max_len and num_q_heads as given to it, top 0 for mq_shared_prefix_attention. For
+ * mq_sparse_attention prefix_len is 0 and max_len min(top, width) * page_size. */
 int mq_attention_workspace(const MqPagePool* pool, int num_q_heads, int batch, int prefix_len, int max_len, int top,
                            size_t* bytes);
 
@@ -346,7 +346,8 @@ int mq_sparse_attention(const MqPagePool* pool, const void* q, long long q_sb, l
  *   workspace: 256-byte aligned, mq_decode_batch_workspace's bytes for the same arguments.
  * On return (stream-ordered) output_token_ids[b] = argmax of the bf16 logits (lowest index on ties), or
  * -(1 + flags) and an unchanged lens[b]: flag 1 if its id was outside the vocabulary, 2 if its position
- * was outside the RoPE tables or its page table, 4 if it needed a page outside the pool. Uses no
+ * was outside the RoPE tables or its page table, 4 if it needed a page outside the pool (or its logits
+ * are not numbers); rows behind lens[b] and the bounds of the page they lie in are then unspecified. Uses no
  * library workspace, allocates nothing and can be captured. */
 int mq_decode_batch(const int* input_token_ids, int* output_token_ids, void* logits_output, int batch,
                     const void* embed_weight, const PrefillLayerWeights* layer_weights, const void* final_norm_weight,

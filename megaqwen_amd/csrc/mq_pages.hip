@@ -358,8 +358,8 @@ constexpr float SLACK = 1.f;
 // for V, and the maximum takes three operands (v_maximum3_f32; a score that is not a number
 // makes its row's output not a number either way).
 template <bool F16, int D, int RB, int NT, class BeforeV>
-__device__ __forceinline__ void attend_step(uint32_t kb, uint32_t vb, int left, float scale, float slack, int kg, uint32_t ka, uint32_t va,
-                                            const u32x4 (&qf)[RB][D / 32], float (&m)[RB], f32x4 (&l)[RB],
+__device__ __forceinline__ void attend_step(uint32_t kb, uint32_t vb, int left, float scale, float slack, int kg, uint32_t ka,
+                                            uint32_t va, const u32x4 (&qf)[RB][D / 32], float (&m)[RB], f32x4 (&l)[RB],
                                             f32x4 (&o)[RB][D / 16], BeforeV before_v) {
   f32x4 sc[RB][NT];
   // two key tiles at a time (2 RB chains of products that do not wait for each other); a pair's K fragments are
@@ -1073,7 +1073,8 @@ static void move_launch(const MqPagePool& P, const int* pages, int n, int first,
 template <bool IN>
 static int move(const MqPagePool* P, const int* pages, int length, const void* kc, const void* vc, int max_seq,
                 hipStream_t stream) {
-  if (!pool_ok(P, false) || !pages || !kc || !vc || !aligned16(kc) || !aligned16(vc) || length < 1 || max_seq < length)
+  if (!pool_ok(P, false) || !pages || !kc || !vc || !aligned16(kc) || !aligned16(vc) || length < 1 ||
+      length > MAX_KEYS || max_seq < length)
     return MQ_ERR_ARG;
   const int n = (length + P->page_size - 1) / P->page_size;
   if (!ids_ok(pages, n, P->num_pages)) return MQ_ERR_ARG;
@@ -1304,8 +1305,9 @@ extern "C" int mq_pages_append(const MqPagePool* pool, const void* k, const void
 
 extern "C" int mq_attention_workspace(const MqPagePool* pool, int num_q_heads, int batch, int prefix_len, int max_len, int top,
                                       size_t* bytes) {
-  if (!pool || !bytes || pool->num_kv_heads < 1 || num_q_heads < pool->num_kv_heads || num_q_heads % pool->num_kv_heads ||
-      batch < 1 || prefix_len < 0 || prefix_len > MAX_KEYS || max_len < 0 || max_len > MAX_KEYS || top < 0)
+  if (!pool || !bytes || pool->num_kv_heads < 1 || num_q_heads < pool->num_kv_heads || num_q_heads > 16384 ||
+      num_q_heads % pool->num_kv_heads || batch < 1 || batch > 65535 || prefix_len < 0 || prefix_len > MAX_KEYS || max_len < 0 ||
+      max_len > MAX_KEYS || top < 0 || top > MQ_MAX_TABLE_WIDTH)
     return MQ_ERR_ARG;
   *bytes = plan_attention(batch, pool->num_kv_heads, num_q_heads / pool->num_kv_heads, pool->head_dim, prefix_len, max_len).bytes +
            (top > 0 ? chosen_bytes(batch, pool->num_kv_heads, top) : 0);

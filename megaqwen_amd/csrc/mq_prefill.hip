@@ -2271,7 +2271,8 @@ static BatchBufs batch_bufs(int batch, int prefix_len, int max_len, int top, int
 static bool batch_args_ok(const MqPagePool* P, int batch, int prefix_len, int max_len, int top, int width) {
   return P && P->num_kv_heads == NKV && P->head_dim == HD && P->dtype == MQ_BF16 && P->num_layers >= 1 &&
          P->num_layers <= MAX_LAYERS && P->page_size >= 16 && P->page_size <= 256 && (P->page_size & (P->page_size - 1)) == 0 &&
-         batch >= 1 && batch <= MAX_BATCH && prefix_len >= 0 && prefix_len <= 1 << 30 && max_len >= 1 && max_len <= 1 << 30 && top >= 0 && top <= MQ_MAX_TABLE_WIDTH &&
+         batch >= 1 && batch <= MAX_BATCH && prefix_len >= 0 && prefix_len <= 1 << 30 && max_len >= 1 && max_len <= 1 << 30 &&
+         top >= 0 && top <= MQ_MAX_TABLE_WIDTH &&
          (top == 0 || (prefix_len == 0 && P->bounds)) && width >= 1 && width <= MQ_MAX_TABLE_WIDTH;
 }
 
@@ -2288,8 +2289,9 @@ extern "C" int mq_decode_batch(const int* input_token_ids, int* output_token_ids
                                const void* sin_table, int num_positions, const MqPagePool* pool, const int* prefix_pages,
                                int prefix_len, const int* tables, long long table_stride, int width, int* lens, int max_len,
                                int top, float attn_scale, void* workspace, size_t workspace_bytes, hipStream_t stream) {
-  if (!batch_args_ok(pool, batch, prefix_len, max_len, top, width) || !pool->k || !pool->v || pool->num_pages < 1 || !tables ||
-      !lens || !workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || num_positions <= prefix_len || table_stride < 0 ||
+  auto aligned16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  if (!batch_args_ok(pool, batch, prefix_len, max_len, top, width) || !pool->k || !pool->v || !aligned16(pool->k) ||
+      !aligned16(pool->v) || !aligned16(pool->bounds) || pool->num_pages < 1 || !tables || !lens || !workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || num_positions <= prefix_len || table_stride < 0 ||
       (prefix_len > 0 && !prefix_pages) ||
       !prefill_args_ok(input_token_ids, output_token_ids, batch, embed_weight, layer_weights, final_norm_weight, lm_head_weight,
                        cos_table, sin_table, pool->k, pool->v, pool->num_layers, batch, attn_scale))

@@ -179,8 +179,11 @@ def _query(q, out, pool, like) -> tuple[torch.Tensor, tuple[int, int], tuple[int
         sb, sh, _ = out.stride()
         return out, strides, (sb if shape[0] > 1 else 0, sh if shape[1] > 1 else 0)
     out_strides = _rows(out, "out", like, shape)
-    if (shape[0] > 1 and out_strides[0] == 0) or (shape[1] > 1 and out_strides[1] == 0):
-        raise ValueError("out: rows that overlap")
+    span = shape[2]
+    for stride, n in sorted(zip(out_strides, shape)):
+        if n > 1 and stride < span:
+            raise ValueError(f"out: rows that overlap, strides {out.stride()}")
+        span += stride * (n - 1)
     return out, strides, out_strides
 
 

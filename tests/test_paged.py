@@ -201,6 +201,29 @@ def test_attention_refusals():
     _refused("on the GPU", sparse, Q, k, k, b, T, LENS, 2)
 
 
+def test_outputs_that_overlap_are_refused():
+    pre, k, b = torch.zeros(2, dtype=torch.int32), K[0], B[0]
+    flat = torch.zeros(4096, dtype=BF)
+    for strides, ok in (((256, 64, 1), True), ((64, 192, 1), True), ((512, 128, 1), True), ((256, 56, 1), False), ((128, 64, 1), False),
+                        ((8, 64, 1), False), ((64, 64, 1), False), ((64, 128, 1), False)):
+        out = flat.as_strided((3, 4, 64), strides)
+        _refused("on the GPU" if ok else "overlap", paged.shared_prefix_attention, Q, k, k, pre, 20, T, LENS, out=out)
+        _refused("on the GPU" if ok else "overlap", paged.sparse_attention, Q, k, k, b, T, LENS, 2, out=out)
+    one = flat.as_strided((1, 4, 64), (8, 64, 1))  # (a stride over one element does not matter)
+    _refused("on the GPU", paged.shared_prefix_attention, Q[:1], k, k, pre, 20, T[:1], LENS[:1], out=one)
+
+
+def test_entries_refuse_what_passes_their_limits():
+    L, n = _abi.lib(), ctypes.c_size_t()
+    ids = (ctypes.c_int * 1)(0)
+    for entry in (L.mq_pages_load, L.mq_pages_store):
+        assert entry(_pool(), ids, 2**31 - 1, 16, 16, 2**31 - 1, None) == _abi.MQ_ERR_ARG
+    for bad in ((_pool(), 16386, 1, 0, 16, 0), (_pool(), 4, 65536, 0, 16, 0), (_pool(), 4, 1, 0, 16, 8193)):
+        assert L.mq_attention_workspace(*bad, n) == _abi.MQ_ERR_ARG
+    for bad in (dict(k=24), dict(v=24), dict(bounds=24)):
+        assert _batch(_model_pool(**bad)) == _abi.MQ_ERR_ARG
+
+
 # ---------------------------------------------------------------- the batched decode step
 
 def _layers(n=2, **over):
