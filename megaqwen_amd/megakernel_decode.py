@@ -505,6 +505,7 @@ class MegakernelBatchDecoder:
         ids = torch.tensor(tokens, dtype=torch.int32).to(dev)
         out = torch.empty(n, dtype=torch.int32, device=dev)
         logits = torch.empty(n, VOCAB_SIZE, dtype=torch.bfloat16, device=dev) if want_logits else None
+        self._key = None  # (the launch changes the lengths on the GPU; an error before the end leaves them unknown)
         paged._call("mq_decode_batch", dev, _ptr(ids), _ptr(out), _ptr(logits), n, _ptr(d.embed_weight_),
                     ctypes.addressof(d.h_layer_weights_), _ptr(d.final_norm_weight_), _ptr(d.lm_head_weight_), _ptr(d.cos_table_),
                     _ptr(d.sin_table_), d.cos_table_.shape[0], pool, _ptr(self.prefix_pages_) if self.prefix_len_ else None,
@@ -853,7 +854,7 @@ class MegakernelPrefillGenerator(_GeneratorBase):
     def _batch(self, n: int, prompt_len: int, max_new_tokens: int, sparse_pages) -> MegakernelBatchDecoder:
         """A batch decoder with room for n continuations; the last one is kept while it is large enough."""
         page = 64
-        each = -(-min(max_new_tokens + 1, self.max_seq_len) // page) + 1  # (the page that the prompt ends in is copied)
+        each = -(-min(max(max_new_tokens, 0) + 1, self.max_seq_len) // page) + 1  # (the page that the prompt ends in is copied)
         need = -(-prompt_len // page) + n * each
         b = getattr(self, "batch_decoder_", None)
         if b is None or b.max_batch < n or b.cache.num_pages < need or b.sparse_pages_ != (sparse_pages or 0):

@@ -179,6 +179,27 @@ def test_rows_that_a_user_appends_between_steps(small):
     _close(got[0], dec.decode_step_with_logits(7)[1])
 
 
+def test_a_step_that_is_cut_short_leaves_no_stale_lengths(small):
+    """An error after the launch, which has advanced the lengths on the GPU: the next step starts from the books."""
+    dec, single = small
+    prompt = weights.random_prompt(40, seed=31)
+    b = MK.MegakernelBatchDecoder(dec, max_batch=2, page_size=16, num_pages=20)
+    seqs = [b.prefill(prompt)[0]]
+    seqs += b.fork(seqs[0])
+    b.step(seqs, [1, 2])
+
+    def cut(*_):
+        raise KeyboardInterrupt
+
+    b.cache.extend = cut
+    with pytest.raises(KeyboardInterrupt):
+        b.step(seqs, [3, 4])
+    del b.cache.extend
+    got, logits = b.step_with_logits(seqs, [5, 6])
+    for i in range(2):
+        _close(logits[i], _expect(single, list(prompt) + [1 + i, 5 + i])[1], got[i])
+
+
 def test_step_refusals(small):
     dec, _ = small
     b = MK.MegakernelBatchDecoder(dec, max_batch=2, page_size=16, num_pages=3)
