@@ -57,19 +57,18 @@ def _pool(k_pages, v_pages, bounds, layered: bool) -> _abi.MqPagePool:
         raise ValueError(f"k_pages: expected a tensor of {dims} dimensions, bfloat16 or float16")
     shape, dtype, device = k_pages.shape, k_pages.dtype, k_pages.device
     _like(v_pages, "v_pages", dtype, device, shape)
-    pages, heads, page, d = shape[-4:]
-    if page not in PAGE_SIZES or d not in HEAD_DIMS or pages == 0 or heads == 0 or shape[0] == 0:
+    layers, pages, heads, page, d = shape if layered else (1, *shape)
+    if page not in PAGE_SIZES or d not in HEAD_DIMS or pages == 0 or heads == 0 or layers == 0:
         raise ValueError(f"k_pages: page size {page} (of {PAGE_SIZES}) or head dim {d} (of {HEAD_DIMS}) or a size of zero")
-    if not k_pages.is_contiguous() or not v_pages.is_contiguous():
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
         raise ValueError("k_pages, v_pages: expected contiguous tensors")
     at = None
     if bounds is not None:
-        _like(bounds, "bounds", dtype, device, shape[:-2] + (2, d))
+        _like(bounds, "bounds", dtype, device, (layers, pages, heads, 2, d) if layered else (pages, heads, 2, d))
         if not bounds.is_contiguous():
             raise ValueError("bounds: expected a contiguous tensor")
         at = bounds.data_ptr()
-    return _abi.MqPagePool(k_pages.data_ptr(), v_pages.data_ptr(), at, shape[0] if layered else 1, pages, heads, page, d,
-                           _DTYPES[dtype])
+    return _abi.MqPagePool(k_pages.data_ptr(), v_pages.data_ptr(), at, layers, pages, heads, page, d, _DTYPES[dtype])
 
 
 def _page_list(ids, name: str, num_pages: int):
@@ -128,28 +127,31 @@ def store_pages(k_pages, v_pages, pages, length: int, k_cache, v_cache) -> None:
     _move("mq_pages_store", k_cache, v_cache, k_pages, v_pages, pages, length, None)
 
 
-def _rows(t, name: str, like, shape) -> tuple[int, int]:
+def _rows(t, name: str, dtype, device, shape) -> tuple[int, int]:
     """(batch, head) strides in elements of a [batch, heads, d] tensor of the pool's type."""
-    _like(t, name, like.dtype, like.device, shape)
+    _like(t, name, dtype, device, shape)
     sb, sh, sd = t.stride()
     # (a stride over one element is never used, whatever it says)
-    sb, sh = (sb if shape[0] > 1 else 0), (sh if shape[1] > 1 else 0)
-    if not (sd == 1 and sb >= 0 and sh >= 0 and sb % 8 == 0 and sh % 8 == 0 and t.data_ptr() % 16 == 0):
+    if shape[0] == 1:
+        sb = 0
+    if shape[1] == 1:
+        sh = 0
+    if not (sd == 1 and sb >= 0 and sh >= 0 and (sb | sh) & 7 == 0 and t.data_ptr() & 15 == 0):
         raise ValueError(f"{name}: expected rows of contiguous elements that begin at multiples of 16 bytes, got strides {t.stride()}")
     return sb, sh
 
 
 def _tables(tables, lens, batch: int, device) -> tuple[int, int]:
     """(row stride, width) of int32 page tables [batch, width]."""
-    if not (isinstance(tables, torch.Tensor) and tables.dim() == 2 and tables.shape[0] == batch
-            and 1 <= tables.shape[1] <= _abi.MQ_MAX_TABLE_WIDTH):
+    n, width = tables.shape if isinstance(tables, torch.Tensor) and tables.dim() == 2 else (0, 0)
+    if n != batch or not 1 <= width <= _abi.MQ_MAX_TABLE_WIDTH:
         raise ValueError(f"tables: expected int32 [{batch}, 1 .. {_abi.MQ_MAX_TABLE_WIDTH}]")
     _like(tables, "tables", torch.int32, device)
     _like(lens, "lens", torch.int32, device, (batch,))
-    width = tables.shape[1]
-    if not ((width == 1 or tables.stride(1) == 1) and (batch == 1 or lens.stride(0) == 1) and tables.stride(0) >= 0):
+    row, entry = tables.stride()
+    if (width > 1 and entry != 1) or (batch > 1 and (row < 0 or lens.stride(0) != 1)):
         raise ValueError("tables, lens: expected contiguous rows")
-    return (tables.stride(0) if batch > 1 else 0), width
+    return (row if batch > 1 else 0), width
 
 
 def append_rows(k, v, k_pages, v_pages, tables, lens, bounds=None) -> None:
@@ -160,31 +162,33 @@ def append_rows(k, v, k_pages, v_pages, tables, lens, bounds=None) -> None:
     pool = _pool(k_pages, v_pages, bounds, False)
     if not (isinstance(k, torch.Tensor) and k.dim() == 3 and 1 <= k.shape[0] <= 65535):
         raise ValueError("k: expected [batch, kv heads, head dim]")
-    shape = (k.shape[0], pool.num_kv_heads, pool.head_dim)
-    k_sb, k_sh = _rows(k, "k", k_pages, shape)
-    v_sb, v_sh = _rows(v, "v", k_pages, shape)
-    t_sb, width = _tables(tables, lens, shape[0], k_pages.device)
-    _call("mq_pages_append", k_pages.device, pool, k.data_ptr(), v.data_ptr(), k_sb, k_sh, v_sb, v_sh, tables.data_ptr(), t_sb,
-          width, lens.data_ptr(), shape[0])
+    batch, dtype, device = k.shape[0], k_pages.dtype, k_pages.device
+    shape = (batch, pool.num_kv_heads, pool.head_dim)
+    k_sb, k_sh = _rows(k, "k", dtype, device, shape)
+    v_sb, v_sh = _rows(v, "v", dtype, device, shape)
+    t_sb, width = _tables(tables, lens, batch, device)
+    _call("mq_pages_append", device, pool, k.data_ptr(), v.data_ptr(), k_sb, k_sh, v_sb, v_sh, tables.data_ptr(), t_sb, width,
+          lens.data_ptr(), batch)
 
 
-def _query(q, out, pool, like) -> tuple[torch.Tensor, tuple[int, int], tuple[int, int]]:
-    if not (isinstance(q, torch.Tensor) and q.dim() == 3 and 1 <= q.shape[0] <= 65535 and 0 < q.shape[1] <= 16384
-            and q.shape[1] % pool.num_kv_heads == 0):
+def _query(q, out, pool, dtype, device):
+    """(shape, out, q's (batch, head) strides, out's) of an attention call."""
+    shape = tuple(q.shape) if isinstance(q, torch.Tensor) else ()
+    if not (len(shape) == 3 and 1 <= shape[0] <= 65535 and 0 < shape[1] <= 16384 and shape[1] % pool.num_kv_heads == 0
+            and shape[2] == pool.head_dim):
         raise ValueError(f"q: expected [batch, a multiple of {pool.num_kv_heads} heads, {pool.head_dim}]")
-    shape = (q.shape[0], q.shape[1], pool.head_dim)
-    strides = _rows(q, "q", like, shape)
+    strides = _rows(q, "q", dtype, device, shape)
     if out is None:
         out = torch.empty_like(q)
         sb, sh, _ = out.stride()
-        return out, strides, (sb if shape[0] > 1 else 0, sh if shape[1] > 1 else 0)
-    out_strides = _rows(out, "out", like, shape)
+        return shape, out, strides, (sb if shape[0] > 1 else 0, sh if shape[1] > 1 else 0)
+    out_strides = _rows(out, "out", dtype, device, shape)
     span = shape[2]
     for stride, n in sorted(zip(out_strides, shape)):
         if n > 1 and stride < span:
             raise ValueError(f"out: rows that overlap, strides {out.stride()}")
         span += stride * (n - 1)
-    return out, strides, out_strides
+    return shape, out, strides, out_strides
 
 
 def _scale(scale, head_dim: int) -> float:
@@ -214,14 +218,14 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix_pages, prefix_len: int, 
     `lens`, if the caller knows it (default width * page size): it decides how the work is split, not what is
     computed. `scale` defaults to 1 / sqrt(head dim)."""
     pool = _pool(k_pages, v_pages, None, False)
-    out, (q_sb, q_sh), (o_sb, o_sh) = _query(q, out, pool, k_pages)
-    batch, heads = q.shape[0], q.shape[1]
-    t_sb, width = _tables(tables, lens, batch, k_pages.device)
+    device = k_pages.device
+    (batch, heads, d), out, (q_sb, q_sh), (o_sb, o_sh) = _query(q, out, pool, k_pages.dtype, device)
+    t_sb, width = _tables(tables, lens, batch, device)
     prefix_len = int(prefix_len)
     if prefix_len < 0:
         raise ValueError("prefix_len must not be negative")
     if prefix_len:
-        _like(prefix_pages, "prefix_pages", torch.int32, k_pages.device)
+        _like(prefix_pages, "prefix_pages", torch.int32, device)
         if not (prefix_pages.dim() == 1 and prefix_pages.is_contiguous()
                 and prefix_pages.numel() >= -(-prefix_len // pool.page_size)):
             raise ValueError(f"prefix_pages: expected at least {-(-prefix_len // pool.page_size)} contiguous page ids")
@@ -229,11 +233,11 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix_pages, prefix_len: int, 
     max_len = whole if max_len is None else min(int(max_len), whole)
     if max_len < 1:
         raise ValueError("max_len must be positive")
-    ws_bytes = _workspace_bytes(pool.num_kv_heads, pool.head_dim, heads, batch, prefix_len, max_len, 0)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
-    _call("mq_shared_prefix_attention", k_pages.device, pool, q.data_ptr(), q_sb, q_sh, out.data_ptr(), o_sb, o_sh, heads, batch,
+    ws_bytes = _workspace_bytes(pool.num_kv_heads, d, heads, batch, prefix_len, max_len, 0)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
+    _call("mq_shared_prefix_attention", device, pool, q.data_ptr(), q_sb, q_sh, out.data_ptr(), o_sb, o_sh, heads, batch,
           prefix_pages.data_ptr() if prefix_len else None, prefix_len, tables.data_ptr(), t_sb, width, lens.data_ptr(), max_len,
-          _scale(scale, pool.head_dim), ws.data_ptr() if ws_bytes else None, ws_bytes)
+          _scale(scale, d), ws.data_ptr() if ws_bytes else None, ws_bytes)
     return out
 
 
@@ -250,16 +254,16 @@ def sparse_attention(q, k_pages, v_pages, bounds, tables, lens, top_pages: int, 
     if bounds is None:
         raise ValueError("bounds: expected a tensor")
     pool = _pool(k_pages, v_pages, bounds, False)
-    out, (q_sb, q_sh), (o_sb, o_sh) = _query(q, out, pool, k_pages)
-    batch, heads, top = q.shape[0], q.shape[1], int(top_pages)
-    t_sb, width = _tables(tables, lens, batch, k_pages.device)
+    device, top = k_pages.device, int(top_pages)
+    (batch, heads, d), out, (q_sb, q_sh), (o_sb, o_sh) = _query(q, out, pool, k_pages.dtype, device)
+    t_sb, width = _tables(tables, lens, batch, device)
     if not 1 <= top <= _abi.MQ_MAX_TABLE_WIDTH:
         raise ValueError(f"top_pages must be in [1, {_abi.MQ_MAX_TABLE_WIDTH}]")
-    chosen = torch.empty(batch, pool.num_kv_heads, top, dtype=torch.int32, device=q.device)
-    ws_bytes = _workspace_bytes(pool.num_kv_heads, pool.head_dim, heads, batch, 0, min(top, width) * pool.page_size, top)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
-    _call("mq_sparse_attention", k_pages.device, pool, q.data_ptr(), q_sb, q_sh, out.data_ptr(), o_sb, o_sh, chosen.data_ptr(), heads,
-          batch, tables.data_ptr(), t_sb, width, lens.data_ptr(), top, _scale(scale, pool.head_dim), ws.data_ptr(), ws_bytes)
+    chosen = torch.empty(batch, pool.num_kv_heads, top, dtype=torch.int32, device=device)
+    ws_bytes = _workspace_bytes(pool.num_kv_heads, d, heads, batch, 0, min(top, width) * pool.page_size, top)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
+    _call("mq_sparse_attention", device, pool, q.data_ptr(), q_sb, q_sh, out.data_ptr(), o_sb, o_sh, chosen.data_ptr(), heads,
+          batch, tables.data_ptr(), t_sb, width, lens.data_ptr(), top, _scale(scale, d), ws.data_ptr(), ws_bytes)
     return out, chosen
 
 
