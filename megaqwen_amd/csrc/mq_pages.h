@@ -29,6 +29,7 @@ struct AttnArgs {
   int64_t t_sb, t_sh;  // table of (sequence, kv head)
   float* part_o;       // [np + ns, batch, hq, d] and (maximum, sum) [np + ns, batch, hq]
   float2* part_ml;
+  uint32_t* tickets;  // [batch, hkv, own_tiles], zero (OWN only)
   int num_pages, hkv, hq, g, lp, width, batch;
   int prefix_len, len_add;  // len_add: rows appended since lens was written
   int prefix_tiles, np, own_tiles, ns;
@@ -40,7 +41,8 @@ struct SelectArgs {
   int64_t q_sb, q_sh, t_sb;
   const int *tables, *lens;
   int *chosen, *pages, *sub_lens;  // [batch, hkv, top] logical and physical, [batch] rows in them
-  int num_pages, hkv, g, lp, width, top, len_add;
+  uint32_t* tickets;               // [batch, hkv, own_tiles], cleared here
+  int num_pages, hkv, g, lp, width, top, len_add, own_tiles;
 };
 
 // How an attention call is split: the form and number of the prefix's row tiles, parts of the

@@ -480,19 +480,36 @@ __device__ __forceinline__ void load_q(const AttnArgs& A, int h, int b0, int row
     for (int ks = 0; ks < D / 32; ks++) settled(qf[rb][ks]);
 }
 
-// Where row r's result goes: part `slot` of the partial results, or, as the only part, the output.
-template <bool F16, int D>
-__device__ __forceinline__ void store_o(const AttnArgs& A, int slot, int h, int b0, int r, int d0, f32x4 x, float m, float l) {
+// Device-scope accesses, for what one workgroup leaves to another of the same launch, maybe on another XCD: they pass
+// the L2, which holds no other XCD's stores.
+__device__ __forceinline__ void put_dev(void* p, u32x2 x) {
+  __hip_atomic_store(static_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ u32x2 get_dev(const void* p) {
+  return __builtin_bit_cast(u32x2, __hip_atomic_load(static_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
+// Where row r's result goes: part `slot` of the partial results, or, as the only part, the output. DEV: the parts are
+// joined in the same launch.
+template <bool F16, int D, bool DEV>
+__device__ __forceinline__ void store_o(const AttnArgs& A, int slot, bool only, int h, int b0, int r, int d0, f32x4 x, float m,
+                                        float l) {
   const int b = b0 + r / A.g, hq = h * A.g + r % A.g;
-  if (A.np + A.ns == 1) {
+  if (only) {
     const float inv = l == 0.f ? 0.f : 1.0f / l;
     *reinterpret_cast<u32x2*>(A.out + (size_t)b * A.o_sb + (size_t)hq * A.o_sh + d0) =
         u32x2{pack2<F16>(x[0] * inv, x[1] * inv), pack2<F16>(x[2] * inv, x[3] * inv)};
     return;
   }
   const size_t at = ((size_t)slot * A.batch + b) * A.hq + hq;
-  *reinterpret_cast<f32x4*>(A.part_o + at * D + d0) = x;
-  if (d0 == 0) A.part_ml[at] = make_float2(m, l);
+  if constexpr (DEV) {
+    put_dev(A.part_o + at * D + d0, u32x2{__float_as_uint(x[0]), __float_as_uint(x[1])});
+    put_dev(A.part_o + at * D + d0 + 2, u32x2{__float_as_uint(x[2]), __float_as_uint(x[3])});
+    if (d0 == 0) put_dev(A.part_ml + at, u32x2{__float_as_uint(m), __float_as_uint(l)});
+  } else {
+    *reinterpret_cast<f32x4*>(A.part_o + at * D + d0) = x;
+    if (d0 == 0) A.part_ml[at] = make_float2(m, l);
+  }
 }
 
 // A run of keys: positions [lo, hi) of the sequence (or prefix) with page table `table`
@@ -505,9 +522,9 @@ struct Run {
 // other until the end: each has 16 KB of LDS, half for K and half for V, and asks for the next step's K as soon as
 // it has the scores of this one, for its V once this one's is multiplied. The rows are read once
 // (or, of several runs, by few workgroups), past the caches: non-temporal, 6.1 against 5.4 TB/s.
-template <bool F16, int D, int RB, int N>
+template <bool F16, int D, int RB, int N, bool DEV>
 __device__ __forceinline__ void own_part(const AttnArgs& A, const Run (&runs)[N], int h, int b0, int row0, int rows, int slot,
-                                         uint32_t lds, float (*s_m)[64], float (*s_l)[64]) {
+                                         bool only, uint32_t lds, float (*s_m)[64], float (*s_l)[64]) {
   constexpr uint32_t HALF = KS * D * 2, WAVE = 2 * HALF;  // bytes of a step's K (or V), and of a wave
   constexpr int NI = KS * D * 2 / 1024;                   // DMA instructions of a step's K (or V)
   static_assert(RB * 16 * D * 4 <= (int)WAVE, "a wave's output fits its LDS");
@@ -616,7 +633,7 @@ __device__ __forceinline__ void own_part(const AttnArgs& A, const Run (&runs)[N]
       const float mw = s_m[w][r], lw = s_l[w][r];
       sum += lw == 0.f ? 0.f : lw * __builtin_amdgcn_exp2f(mw - (mx == -INFINITY ? 0.f : mx));
     }
-    store_o<F16, D>(A, slot, h, b0, row0 + r, 4 * p, x, mx, sum);
+    store_o<F16, D, DEV>(A, slot, only, h, b0, row0 + r, 4 * p, x, mx, sum);
   }
 }
 
@@ -629,7 +646,8 @@ __device__ __forceinline__ void own_part(const AttnArgs& A, const Run (&runs)[N]
 // Without any K and V fetched the steps took 1.6 us where they take 2.35; asking for K and V half a step earlier,
 // with a second barrier, or putting the exponentials of one half between the products of the other gained nothing.
 template <bool F16, int D, int RB>
-__device__ __forceinline__ void prefix_part(const AttnArgs& A, int h, int row0, int rows, int k_lo, int k_hi, int slot, uint32_t lds) {
+__device__ __forceinline__ void prefix_part(const AttnArgs& A, int h, int row0, int rows, int k_lo, int k_hi, int slot, bool only,
+                                            uint32_t lds) {
   constexpr uint32_t HALF = TS * D * 2, STAGE = 2 * HALF;
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, kg = lane >> 4;
   const Lanes<D, false> lk(lane);
@@ -669,7 +687,7 @@ __device__ __forceinline__ void prefix_part(const AttnArgs& A, int h, int row0, 
     const float sum = bad ? NAN : l[rb][0];
     if (r < rows)
 #pragma unroll
-      for (int dt = 0; dt < D / 16; dt++) store_o<F16, D>(A, slot, h, 0, r, 16 * dt + 4 * kg, o[rb][dt], m[rb], sum);
+      for (int dt = 0; dt < D / 16; dt++)         store_o<F16, D, false>(A, slot, only, h, 0, r, 16 * dt + 4 * kg, o[rb][dt], m[rb], sum);
   }
 }
 
@@ -685,74 +703,49 @@ __host__ __device__ __forceinline__ int part_keys(int len, int parts) { return (
 
 // How the query rows of a prefix are tiled: up to 32 rows, all keys' work is split among the waves (own_part);
 // more rows are (prefix_part). JOINED: no tiles of the prefix; each sequence's workgroup goes over the prefix and
-// then over its own rows, so that nothing is left to join and the call is one launch.
-enum : int { ROWS16 = 0, ROWS32 = 1, ROWS64 = 2, ROWS128 = 3, JOINED = 4 };
+// then over its own rows, so that nothing is left to join and the call is one launch. OWN: no prefix, and the last
+// workgroup of a sequence's parts joins them (a launch before has cleared the tickets that tell which one is last): the
+// GPU's time is that of a second launch (one sequence over 64 of 250 pages 15.8 us, 16.0 with it), the host's 4 us less.
+enum : int { ROWS16 = 0, ROWS32 = 1, ROWS64 = 2, ROWS128 = 3, JOINED = 4, OWN = 5 };
 __host__ __device__ constexpr int tile_rows(int form) { return 16 << form; }
 
-template <bool F16, int D, int FORM>
-__global__ void __launch_bounds__(64 * AW, 2) attn_kernel(AttnArgs A) {
-  __shared__ __align__(1024) uint8_t s_kv[4 * TS * D * 2];
-  __shared__ float s_m[AW][64], s_l[AW][64];
-  static_assert(sizeof(s_kv) == AW * 2 * KS * D * 2, "the two forms take the same LDS");
-  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&s_kv[0];
-  if constexpr (FORM == JOINED) {
-    const int h = blockIdx.x % A.hkv, id = blockIdx.x / A.hkv, tile = id % A.own_tiles, b = id / A.own_tiles;
-    const int len = own_rows(A.lens, b, A.len_add, A.width, A.lp);
-    const Run runs[2] = {{A.prefix_pages, 0, A.prefix_len}, {A.tables + (size_t)b * A.t_sb + (size_t)h * A.t_sh, 0, len}};
-    own_part<F16, D, 1>(A, runs, h, b, 16 * tile, A.g, 0, lds, s_m, s_l);
-  } else {
-    // parts of the prefix and of own rows alternate, a workgroup a CU of each, while there are both
-    const int n_prefix = A.hkv * A.prefix_tiles * A.np, n_own = A.hkv * A.own_tiles * A.batch * A.ns;
-    const int runs = min(n_prefix, n_own) / NUM_CUS, bid = blockIdx.x, run = bid / NUM_CUS, rest = bid - runs * NUM_CUS;
-    const bool prefix = run < 2 * runs ? run % 2 == 0 : rest < n_prefix;
-    int id = run < 2 * runs ? run / 2 * NUM_CUS + bid % NUM_CUS : rest < n_prefix ? rest : bid - n_prefix;
-    const int h = id % A.hkv;  // (fastest: with 8 kv heads each XCD reads one head's rows)
-    id /= A.hkv;
-    if (prefix) {
-      const int rows = A.batch * A.g, row0 = tile_rows(FORM) * (id % A.prefix_tiles), part = id / A.prefix_tiles;
-      const int ch = part_keys(A.prefix_len, A.np), lo = part * ch, hi = min(A.prefix_len, lo + ch);
-      if constexpr (FORM <= ROWS32) {
-        const Run mine[1] = {{A.prefix_pages, lo, hi}};
-        own_part<F16, D, FORM == ROWS16 ? 1 : 2>(A, mine, h, 0, row0, rows, part, lds, s_m, s_l);
-      } else {
-        prefix_part<F16, D, FORM == ROWS64 ? 1 : 2>(A, h, row0, rows, lo, hi, part, lds);
-      }
-      return;
-    }
-    const int tile = id % A.own_tiles;
-    id /= A.own_tiles;
-    const int b = id % A.batch, part = id / A.batch;
-    const int len = own_rows(A.lens, b, A.len_add, A.width, A.lp);
-    const int ch = part_keys(len, A.ns), lo = part * ch, hi = min(len, lo + ch);
-    if (lo >= hi) {
-      // no key: the part's sum says so, or, as the only part, the output is zero
-      const int n = min(16, A.g - 16 * tile) * (D / 4);
-      for (int i = threadIdx.x; i < n; i += 64 * AW)
-        if (A.np + A.ns == 1 || i % (D / 4) == 0)
-          store_o<F16, D>(A, A.np + part, h, b, 16 * tile + i / (D / 4), 4 * (i % (D / 4)), f32x4{0.f, 0.f, 0.f, 0.f}, -INFINITY,
-                          0.f);
-      return;
-    }
-    const Run mine[1] = {{A.tables + (size_t)b * A.t_sb + (size_t)h * A.t_sh, lo, hi}};
-    own_part<F16, D, 1>(A, mine, h, b, 16 * tile, A.g, A.np + part, lds, s_m, s_l);
-  }
-}
-
-// A wave a row (query head, sequence): the parts' outputs, scaled to their common maximum, over their sums.
-// Rows without a key give zeros. Lane p takes part p's maximum and sum (and part p + 64's); LPR lanes hold
+// One row (query head, sequence), by one wave: the parts' outputs, scaled to their common maximum, over their sums. Rows
+// without a key give zeros. Lane p takes part p's maximum and sum (and part p + 64's); LPR lanes hold
 // a row's output, and the wave's 64 / LPR groups of them take the parts in turn, eight in flight, and are
-// added in order, so that a result does not depend on timing.
+// added in order, so that a result does not depend on timing. The first eight are asked for together with the maxima,
+// which tell whether a part had a key (if not, its output was not written and is not used). DEV: the parts are of this
+// launch.
 constexpr int MAX_PARTS = 128;
-template <bool F16, int D>
-__global__ void __launch_bounds__(256) combine_kernel(AttnArgs A) {
+template <bool F16, int D, bool DEV>
+__device__ __forceinline__ void join_row(const AttnArgs& A, size_t row, int parts, int lane) {
   constexpr int LPR = D / 4, GROUPS = 64 / LPR, AHEAD = 8;
-  const int lane = threadIdx.x & 63, parts = A.np + A.ns;
-  const size_t rows = (size_t)A.batch * A.hq, row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= rows) return;
+  const size_t rows = (size_t)A.batch * A.hq;
   const int grp = lane / LPR, c = lane % LPR;
-  float2 ml[2];
+  f32x4 y[AHEAD];
+  auto fetch = [&](int p0) {
 #pragma unroll
-  for (int i = 0; i < 2; i++) ml[i] = lane + 64 * i < parts ? A.part_ml[row + rows * (lane + 64 * i)] : make_float2(-INFINITY, 0.f);
+    for (int u = 0; u < AHEAD; u++) {
+      const float* at = A.part_o + (row + rows * min(p0 + GROUPS * u + grp, parts - 1)) * D + 4 * c;
+      if constexpr (DEV) {
+        const u32x2 lo = get_dev(at), hi = get_dev(at + 2);
+        y[u] = __builtin_bit_cast(f32x4, u32x4{lo.x, lo.y, hi.x, hi.y});
+      } else {
+        y[u] = *reinterpret_cast<const f32x4*>(at);
+      }
+    }
+  };
+  float2 ml[2] = {make_float2(-INFINITY, 0.f), make_float2(-INFINITY, 0.f)};
+  if (parts > 0) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const float2* p = A.part_ml + row + rows * min(lane + 64 * i, parts - 1);
+      ml[i] = DEV ? __builtin_bit_cast(float2, get_dev(p)) : *p;
+    }
+    fetch(0);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; i++)
+    if (lane + 64 * i >= parts) ml[i] = make_float2(-INFINITY, 0.f);
   float mx[1] = {fmaxf(ml[0].x, ml[1].x)};
   wave_max_n(mx);
   const float base = mx[0] == -INFINITY ? 0.f : mx[0];
@@ -765,21 +758,17 @@ __global__ void __launch_bounds__(256) combine_kernel(AttnArgs A) {
   }
   l = wave_sum(l);
   f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
   for (int p0 = 0; p0 < parts; p0 += GROUPS * AHEAD) {
-    f32x4 y[AHEAD];
-    float f[AHEAD];
+    if (p0 > 0) fetch(p0);
 #pragma unroll
     for (int u = 0; u < AHEAD; u++) {
       const int p = p0 + GROUPS * u + grp;
-      f[u] = __shfl(p < 64 ? w[0] : w[1], p & 63, 64);
-      if (p >= parts) f[u] = -1.f;
-      y[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (f[u] >= 0.f || f[u] != f[u]) y[u] = *reinterpret_cast<const f32x4*>(A.part_o + (row + rows * p) * D + 4 * c);
+      const float f = __shfl(p < 64 ? w[0] : w[1], p & 63, 64);
+      if (p < parts && !(f < 0.f))
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] += f * y[u][e];
     }
-#pragma unroll
-    for (int u = 0; u < AHEAD; u++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) x[e] += f[u] * y[u][e];
   }
 #pragma unroll
   for (int e = 0; e < 4; e++) {
@@ -790,6 +779,93 @@ __global__ void __launch_bounds__(256) combine_kernel(AttnArgs A) {
   const float inv = l == 0.f ? 0.f : 1.0f / l;
   *reinterpret_cast<u32x2*>(A.out + row / A.hq * A.o_sb + row % A.hq * A.o_sh + 4 * c) =
       u32x2{pack2<F16>(x[0] * inv, x[1] * inv), pack2<F16>(x[2] * inv, x[3] * inv)};
+}
+
+template <bool F16, int D, int FORM>
+__global__ void __launch_bounds__(64 * AW, 2) attn_kernel(AttnArgs A) {
+  __shared__ __align__(1024) uint8_t s_kv[4 * TS * D * 2];
+  __shared__ float s_m[AW][64], s_l[AW][64];
+  static_assert(sizeof(s_kv) == AW * 2 * KS * D * 2, "the two forms take the same LDS");
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&s_kv[0];
+  if constexpr (FORM == JOINED) {
+    const int h = blockIdx.x % A.hkv, id = blockIdx.x / A.hkv, tile = id % A.own_tiles, b = id / A.own_tiles;
+    const int len = own_rows(A.lens, b, A.len_add, A.width, A.lp);
+    const Run runs[2] = {{A.prefix_pages, 0, A.prefix_len}, {A.tables + (size_t)b * A.t_sb + (size_t)h * A.t_sh, 0, len}};
+    own_part<F16, D, 1, 2, false>(A, runs, h, b, 16 * tile, A.g, 0, true, lds, s_m, s_l);
+  } else if constexpr (FORM == OWN) {
+    int id = blockIdx.x;
+    const int h = id % A.hkv;
+    id /= A.hkv;
+    const int tile = id % A.own_tiles;
+    id /= A.own_tiles;
+    const int b = id % A.batch, part = id / A.batch, rows = min(16, A.g - 16 * tile), tid = threadIdx.x;
+    const int len = own_rows(A.lens, b, A.len_add, A.width, A.lp);
+    const int ch = part_keys(len, A.ns), lo = part * ch, hi = min(len, lo + ch);
+    if (lo >= hi) {
+      if (part > 0) return;  // (the parts that have a key are joined)
+      for (int i = tid; i < rows * (D / 4); i += 64 * AW)
+        store_o<F16, D, true>(A, 0, true, h, b, 16 * tile + i / (D / 4), 4 * (i % (D / 4)), f32x4{0.f, 0.f, 0.f, 0.f}, 0.f, 0.f);
+      return;
+    }
+    const int parts = (len + ch - 1) / ch;
+    const Run mine[1] = {{A.tables + (size_t)b * A.t_sb + (size_t)h * A.t_sh, lo, hi}};
+    own_part<F16, D, 1, 1, true>(A, mine, h, b, 16 * tile, A.g, part, parts == 1, lds, s_m, s_l);
+    if (parts == 1) return;
+    PG_AWAIT(0);  // the wave's stores have been written, and after the barrier every wave's
+    __shared__ int s_last;
+    __syncthreads();
+    if (tid == 0)
+      s_last = __hip_atomic_fetch_add(A.tickets + ((size_t)b * A.hkv + h) * A.own_tiles + tile, 1u, __ATOMIC_RELAXED,
+                                      __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)parts - 1;
+    __syncthreads();
+    if (!s_last) return;
+    for (int r = tid >> 6; r < rows; r += AW)
+      join_row<F16, D, true>(A, (size_t)b * A.hq + h * A.g + 16 * tile + r, parts, tid & 63);
+  } else {
+    // parts of the prefix and of own rows alternate, a workgroup a CU of each, while there are both
+    const bool only = A.np + A.ns == 1;
+    const int n_prefix = A.hkv * A.prefix_tiles * A.np, n_own = A.hkv * A.own_tiles * A.batch * A.ns;
+    const int runs = min(n_prefix, n_own) / NUM_CUS, bid = blockIdx.x, run = bid / NUM_CUS, rest = bid - runs * NUM_CUS;
+    const bool prefix = run < 2 * runs ? run % 2 == 0 : rest < n_prefix;
+    int id = run < 2 * runs ? run / 2 * NUM_CUS + bid % NUM_CUS : rest < n_prefix ? rest : bid - n_prefix;
+    const int h = id % A.hkv;  // (fastest: with 8 kv heads each XCD reads one head's rows)
+    id /= A.hkv;
+    if (prefix) {
+      const int rows = A.batch * A.g, row0 = tile_rows(FORM) * (id % A.prefix_tiles), part = id / A.prefix_tiles;
+      const int ch = part_keys(A.prefix_len, A.np), lo = part * ch, hi = min(A.prefix_len, lo + ch);
+      if constexpr (FORM <= ROWS32) {
+        const Run mine[1] = {{A.prefix_pages, lo, hi}};
+        own_part<F16, D, FORM == ROWS16 ? 1 : 2, 1, false>(A, mine, h, 0, row0, rows, part, only, lds, s_m, s_l);
+      } else {
+        prefix_part<F16, D, FORM == ROWS64 ? 1 : 2>(A, h, row0, rows, lo, hi, part, only, lds);
+      }
+      return;
+    }
+    const int tile = id % A.own_tiles;
+    id /= A.own_tiles;
+    const int b = id % A.batch, part = id / A.batch;
+    const int len = own_rows(A.lens, b, A.len_add, A.width, A.lp);
+    const int ch = part_keys(len, A.ns), lo = part * ch, hi = min(len, lo + ch);
+    if (lo >= hi) {
+      // no key: the part's sum says so, or, as the only part, the output is zero
+      const int n = min(16, A.g - 16 * tile) * (D / 4);
+      for (int i = threadIdx.x; i < n; i += 64 * AW)
+        if (only || i % (D / 4) == 0)
+          store_o<F16, D, false>(A, A.np + part, only, h, b, 16 * tile + i / (D / 4), 4 * (i % (D / 4)), f32x4{0.f, 0.f, 0.f, 0.f},
+                                 -INFINITY, 0.f);
+      return;
+    }
+    const Run mine[1] = {{A.tables + (size_t)b * A.t_sb + (size_t)h * A.t_sh, lo, hi}};
+    own_part<F16, D, 1, 1, false>(A, mine, h, b, 16 * tile, A.g, A.np + part, only, lds, s_m, s_l);
+  }
+}
+
+// A wave a row.
+template <bool F16, int D>
+__global__ void __launch_bounds__(256) combine_kernel(AttnArgs A) {
+  const size_t row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= (size_t)A.batch * A.hq) return;
+  join_row<F16, D, false>(A, row, A.np + A.ns, threadIdx.x & 63);
 }
 
 // ------------------------------------------------------------------ choosing pages
@@ -879,6 +955,7 @@ __global__ void __launch_bounds__(ST) select_kernel(SelectArgs A) {
   int* chosen = A.chosen + ((size_t)b * A.hkv + h) * A.top;
   int* pages = A.pages + ((size_t)b * A.hkv + h) * A.top;
   const int count = min(used, A.top), n = used - 1;  // n: pages with a score
+  if (tid < A.own_tiles) A.tickets[((size_t)b * A.hkv + h) * A.own_tiles + tid] = 0;
   if (h == 0 && tid == 0) A.sub_lens[b] = count == 0 ? 0 : ((count - 1) << A.lp) + ((len - 1) & ((1 << A.lp) - 1)) + 1;
   for (int i = count + tid; i < A.top; i += ST) chosen[i] = -1, pages[i] = -1;
   if (used <= A.top) {
@@ -1159,13 +1236,14 @@ static void attn_launch(const AttnArgs& A, int form, unsigned blocks, hipStream_
       case ROWS32: attn_kernel<F16, D, ROWS32><<<blocks, 64 * AW, 0, stream>>>(A); break;
       case ROWS64: attn_kernel<F16, D, ROWS64><<<blocks, 64 * AW, 0, stream>>>(A); break;
       case JOINED: attn_kernel<F16, D, JOINED><<<blocks, 64 * AW, 0, stream>>>(A); break;
+      case OWN: attn_kernel<F16, D, OWN><<<blocks, 64 * AW, 0, stream>>>(A); return;
       default: attn_kernel<F16, D, ROWS128><<<blocks, 64 * AW, 0, stream>>>(A); break;
     }
   }
   if (A.np + A.ns != 1) combine_kernel<F16, D><<<((unsigned)A.batch * A.hq + 3) / 4, 256, 0, stream>>>(A);
 }
 
-// Both launches of an attention; A without its split and partial results, which come from `p` and
+// The launches of an attention; A without its split and partial results, which come from `p` and
 // `ws` (plan_attention's bytes).
 int run_attention(AttnArgs A, const AttnPlan& p, int d, bool f16, void* ws, hipStream_t stream) {
   A.prefix_tiles = p.prefix_tiles; A.np = p.np; A.own_tiles = p.own_tiles; A.ns = p.ns;
@@ -1221,11 +1299,13 @@ int shared_attention(const MqPagePool* P, const void* q, int64_t q_sb, int64_t q
   return run_attention(A, p, P->head_dim, P->dtype == MQ_FP16, ws, stream);
 }
 
-// The chosen pages and the rows in them, ahead of the attention's partial results in the workspace.
-static size_t chosen_bytes(int batch, int hkv, int top) { return ((size_t)batch * (hkv * (size_t)top + 1) * 4 + 255) / 256 * 256; }
+// The chosen pages, the rows in them and the tickets, ahead of the attention's partial results in the workspace.
+static size_t chosen_bytes(int batch, int hkv, int g, int top) {
+  return ((size_t)batch * (hkv * ((size_t)top + (g + 15) / 16) + 1) * 4 + 255) / 256 * 256;
+}
 
 size_t sparse_workspace(int batch, int hkv, int g, int d, int top, int width, int page_size) {
-  return chosen_bytes(batch, hkv, top) + plan_attention(batch, hkv, g, d, 0, (top < width ? top : width) * page_size).bytes;
+  return chosen_bytes(batch, hkv, g, top) + plan_attention(batch, hkv, g, d, 0, (top < width ? top : width) * page_size).bytes;
 }
 
 int sparse_attention(const MqPagePool* P, const void* q, int64_t q_sb, int64_t q_sh, void* out, int64_t o_sb, int64_t o_sh,
@@ -1235,14 +1315,16 @@ int sparse_attention(const MqPagePool* P, const void* q, int64_t q_sb, int64_t q
       top < 1 || top > MQ_MAX_TABLE_WIDTH)
     return MQ_ERR_ARG;
   const int most = top < width ? top : width, hkv = P->num_kv_heads, g = num_q_heads / hkv;
-  const AttnPlan p = plan_attention(batch, hkv, g, P->head_dim, 0, most * P->page_size);
-  const size_t head = chosen_bytes(batch, hkv, top);
+  AttnPlan p = plan_attention(batch, hkv, g, P->head_dim, 0, most * P->page_size);
+  p.form = OWN;
+  const size_t head = chosen_bytes(batch, hkv, g, top);
   if (!workspace_ok(ws, ws_bytes, head + p.bytes)) return MQ_ERR_ARG;
   AttnArgs A = attn_args(*P, q, q_sb, q_sh, out, o_sb, o_sh, num_q_heads, batch, scale);
   SelectArgs S{};
   S.q = A.q; S.bounds = static_cast<const uint16_t*>(P->bounds);
   S.q_sb = q_sb; S.q_sh = q_sh; S.t_sb = t_sb; S.tables = tables; S.lens = lens;
   S.chosen = chosen; S.pages = static_cast<int*>(ws); S.sub_lens = S.pages + (size_t)batch * hkv * top;
+  S.tickets = reinterpret_cast<uint32_t*>(S.sub_lens + batch); S.own_tiles = p.own_tiles;
   S.num_pages = P->num_pages; S.hkv = hkv; S.g = g; S.lp = A.lp; S.width = width; S.top = top; S.len_add = len_add;
   const dim3 grid(hkv, batch);
   const size_t keys = (size_t)width * 8;
@@ -1253,6 +1335,7 @@ int sparse_attention(const MqPagePool* P, const void* q, int64_t q_sb, int64_t q
     f16 ? select_kernel<true, 64><<<grid, ST, keys, stream>>>(S) : select_kernel<false, 64><<<grid, ST, keys, stream>>>(S);
   if (hipGetLastError() != hipSuccess) return MQ_ERR_HIP;
   A.tables = S.pages; A.t_sb = (int64_t)hkv * top; A.t_sh = top; A.width = top; A.lens = S.sub_lens;
+  A.tickets = S.tickets;
   return run_attention(A, p, P->head_dim, f16, static_cast<char*>(ws) + head, stream);
 }
 
@@ -1310,7 +1393,7 @@ extern "C" int mq_attention_workspace(const MqPagePool* pool, int num_q_heads, i
       max_len > MAX_KEYS || top < 0 || top > MQ_MAX_TABLE_WIDTH)
     return MQ_ERR_ARG;
   *bytes = plan_attention(batch, pool->num_kv_heads, num_q_heads / pool->num_kv_heads, pool->head_dim, prefix_len, max_len).bytes +
-           (top > 0 ? chosen_bytes(batch, pool->num_kv_heads, top) : 0);
+           (top > 0 ? chosen_bytes(batch, pool->num_kv_heads, num_q_heads / pool->num_kv_heads, top) : 0);
   return MQ_OK;
 }
 

@@ -442,6 +442,38 @@ def test_sparse_attention(case):
     _check(out, q, rows_of, 1 / math.sqrt(d))
 
 
+@pytest.mark.parametrize("G,d", [(20, 128), (1, 64), (33, 64)])
+def test_sparse_parts_join_in_a_replayed_graph(G, d):
+    """Sequences of no, one and many parts, whose lengths change between the replays of one graph; all pages are chosen."""
+    from megaqwen_amd import paged
+
+    hkv, page, top = 2, 64, 48
+    lens = [3000, 128, 129, 1500, 3000, 1]
+    q, k, v, _, tables, lens_d, rows_of = _setup(6, hkv, G, d, page, BF, 0, lens, seed=G)
+    bounds = torch.zeros(k.shape[0], hkv, 2, d, dtype=BF, device=DEV)  # (never decides: no sequence has more pages)
+
+    def eager():
+        return paged.sparse_attention(q, k, v, bounds, tables, lens_d, top)[0]
+
+    _check(eager(), q, rows_of, 1 / math.sqrt(d))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = [eager() for _ in range(3)]
+    for now in (lens, [0, 100, 128, 700, 2999, 1], [1280, 1, 0, 1408, 64, 0], lens):
+        lens_d.copy_(torch.tensor(now, dtype=torch.int32))
+        want = eager().clone()
+        for o in outs:
+            o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for o in outs:
+            assert torch.equal(_bits(o), _bits(want))
+        for b, n in enumerate(now):
+            assert n > 0 or not want[b].any()
+    _check(want, q, rows_of, 1 / math.sqrt(d))
+
+
 def test_sparse_choice_of_equal_scores_takes_the_earlier_pages():
     from megaqwen_amd import paged
 
