@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(CT) move_kernel(MoveArgs<N> A) {
 
 // Workgroup b: sequence b's new K and V row to its position lens[b], and the page's bounds: the row
 // itself where it is the page's first, the least and greatest with it otherwise. A position behind
-// the table or a page outside the pool: nothing is written. 2 us for one sequence, 3.2 for 200: length, page id and
+// the table or a page outside the pool: nothing is written. 2 us for one sequence, 3.1 for 200: length, page id and
 // bounds are read one behind the other.
 template <bool F16>
 __global__ void __launch_bounds__(CT) append_kernel(AppendArgs A) {
@@ -877,7 +877,7 @@ __global__ void __launch_bounds__(256) combine_kernel(AttnArgs A) {
 // the order of the additions. Chosen are the last page and the top - 1 best others, the lower
 // of equals first; a score that is not a number counts as the greatest.
 //
-// One workgroup a (kv head, sequence), 7.6 us for 250 pages, of which 2.7 are the sums (128 64-bit conversions
+// One workgroup a (kv head, sequence), 7.5 us for 250 pages, of which 2.7 are the sums (128 64-bit conversions
 // and products a lane on one CU) and 2.3 the choice: 16 lanes take a page (8 dims each at 128), the scores go to LDS
 // as unsigned 64-bit keys in the order of the scores. Of up to 1024 of them one wave finds the last that is
 // chosen, of more the workgroup, by a radix selection 8 bits at a time. The chosen pages are written in
