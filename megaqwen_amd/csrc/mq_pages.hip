@@ -1176,7 +1176,11 @@ int append_rows(const AppendArgs& A, bool f16, hipStream_t stream) {
 }
 
 // How an attention call is split. Query rows of the prefix go in tiles of up to 128, so that its keys are read
-// as few times as there are tiles; a sequence's own rows are shared by its G query heads a kv head only, in
+// as few times as there are tiles; of 64 while there are at most 1024 steps of 128 rows by 64 keys, four a CU: a step
+// then takes half as long, and what a workgroup does one behind the other is what bounds such calls (64 sequences behind
+// 2000 rows with up to 64 own 14.5 us against 17.7, 23 behind 1117 with 5 queries a kv head 8.2 against 9.5; the other
+// way from some 2000 steps on: 128 behind 8192 with up to 500 own 40.8 against 45.8 with tiles of 64, 256 behind 15001
+// with up to 1024 110 against 130). A sequence's own rows are shared by its G query heads a kv head only, in
 // tiles of 16. Keys are split until the launch has about two workgroups a CU, in parts of at least 128 keys.
 // Each part's result is another 4 D + 8 bytes a query row written and read, so tiles of more than 32 rows take fewer
 // parts where those cost nothing (us a captured call):
@@ -1194,6 +1198,7 @@ constexpr int JOINED_KEYS = 640;
 AttnPlan plan_attention(int batch, int hkv, int g, int d, int prefix_len, int max_len) {
   AttnPlan p{};
   constexpr int WANT = 512;
+  constexpr long long HALF_TILES = 1024;
   constexpr double STEP_US = 1.8, SHORT_WANT = 192., SHORT_STEPS = 16.;
   const int rows = batch * g;
   p.own_tiles = (g + 15) / 16;
@@ -1202,7 +1207,8 @@ AttnPlan plan_attention(int batch, int hkv, int g, int d, int prefix_len, int ma
     p.ns = 1;
     return p;
   }
-  p.form = rows <= 16 ? ROWS16 : rows <= 32 ? ROWS32 : rows <= 64 ? ROWS64 : ROWS128;
+  const long long steps128 = (long long)hkv * ((rows + 127) / 128) * ((prefix_len + TS - 1) / TS);
+  p.form = rows <= 16 ? ROWS16 : rows <= 32 ? ROWS32 : rows <= 64 || steps128 <= HALF_TILES ? ROWS64 : ROWS128;
   auto parts = [&](int len, long long tiles, double want) {
     const int most = (len + UNIT - 1) / UNIT;
     double n = ceil(want / (double)tiles);

@@ -291,6 +291,22 @@ def test_shared_prefix_attention(case):
         _check(paged.shared_prefix_attention(q, k, v, pre, prefix, tables, lens_d, max_len=hint), q, rows_of, scale)
 
 
+@pytest.mark.parametrize("case", [
+    # tiles of 128 rows: more than 1024 steps of 64 keys by 128 rows, with a last tile, page, part and step that are not full
+    (40, 16, 4, 128, 64, BF, 2100, [0, 1, 63, 64, 65, 300, 7, 129] * 5),
+    (30, 16, 5, 64, 16, FP, 2113, [0, 200, 16] * 10),
+    (65, 8, 2, 128, 256, FP, 4097, [0] * 65),
+    (65, 16, 2, 64, 128, BF, 2100, [40] * 65),
+], ids=lambda c: f"b{c[0]}h{c[1]}x{c[2]}d{c[3]}p{c[4]}n{c[6]}")
+def test_shared_prefix_attention_of_large_batches(case):
+    from megaqwen_amd import paged
+
+    B, hkv, G, d, page, dtype, prefix, lens = case
+    q, k, v, pre, tables, lens_d, rows_of = _setup(B, hkv, G, d, page, dtype, prefix, lens, seed=B)
+    out = paged.shared_prefix_attention(q, k, v, pre, prefix, tables, lens_d)
+    _check(out, q, rows_of, 1 / math.sqrt(d))
+
+
 def test_shared_prefix_attention_strides_scale_and_out():
     """q and out as slices of wider rows, tables as a slice of whole tables, another scale; repeats are bit-identical."""
     from megaqwen_amd import paged
