@@ -32,7 +32,7 @@ struct AttnArgs {
   uint32_t* tickets;  // [batch, hkv, own_tiles], zero (OWN only)
   int num_pages, hkv, hq, g, lp, width, batch;
   int prefix_len, len_add;  // len_add: rows appended since lens was written
-  int prefix_tiles, np, own_tiles, ns;
+  int prefix_tiles, np, own_tiles, groups, ns;  // groups: of sequences, one or (a wave each) four of them
   float scale_log2;
 };
 
@@ -48,7 +48,7 @@ struct SelectArgs {
 // How an attention call is split: the form and number of the prefix's row tiles, parts of the
 // prefix and of the own rows, and the workspace: the partial outputs, then the maxima and sums.
 struct AttnPlan {
-  int form, prefix_tiles, np, own_tiles, ns;
+  int form, prefix_tiles, np, own_tiles, groups, ns;
   size_t out_bytes, bytes;
 };
 AttnPlan plan_attention(int batch, int hkv, int g, int d, int prefix_len, int max_len);

@@ -518,15 +518,99 @@ struct Run {
   int lo, hi;
 };
 
-// The keys of N runs for up to RB * 16 query rows. The waves take 32-key steps in turn and do not wait for each
-// other until the end: each has 16 KB of LDS, half for K and half for V, and asks for the next step's K as soon as
-// it has the scores of this one, for its V once this one's is multiplied. The rows are read once
-// (or, of several runs, by few workgroups), past the caches: non-temporal, 6.1 against 5.4 TB/s.
+// The 32-key steps of a run from key k0 on, every `stride` keys, by one wave with 16 KB of LDS, half for K and half for
+// V: it asks for the next step's K as soon as it has the scores of this one, for its V once this one's is multiplied.
+// load() brings the query fragments. The rows are read once (or, of several runs, by few workgroups), past the caches:
+// non-temporal, 6.1 against 5.4 TB/s. True if a page was outside the pool.
+template <bool F16, int D, int RB, class Load>
+__device__ __forceinline__ bool walk(const AttnArgs& A, const Run& run, int h, int k0, int stride, uint32_t mine, int lane,
+                                     const Lanes<D, false>& lk, const Lanes<D, true>& lv, u32x4 (&qf)[RB][D / 32],
+                                     float (&m)[RB], f32x4 (&l)[RB], f32x4 (&o)[RB][D / 16], Load load) {
+  constexpr uint32_t HALF = KS * D * 2;  // bytes of a step's K (or V)
+  constexpr int NI = KS * D * 2 / 1024;  // DMA instructions of it
+  const uint32_t ka = k_frag<D>(lane & 15, lane >> 4), va = v_frag<D>(lane & 15, lane >> 4);
+  const int k_hi = run.hi;
+  const bool any = k0 < k_hi;  // (the wave's)
+  Pages pages(run.table, A.num_pages, run.lo >> A.lp, max(run.lo, k_hi - 1) >> A.lp, lane, any);
+  size_t at[2];  // a step's two tiles
+  int last[2];
+  auto find = [&](int k0) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const Tile t(pages, A, h, D, k0 + 16 * i, k_hi - 1, lane);
+      at[i] = t.at;
+      last[i] = t.last;
+    }
+  };
+  auto fetch_k = [&] {
+#pragma unroll
+    for (int i = 0; i < 2; i++) lk.template fetch<true>(A.k + at[i], last[i], mine + HALF / 2 * i, lane);
+  };
+  auto fetch_v = [&] {
+#pragma unroll
+    for (int i = 0; i < 2; i++) lv.template fetch<true>(A.v + at[i], last[i], mine + HALF + HALF / 2 * i, lane);
+  };
+  if (any) {
+    find(k0);
+    fetch_k();
+    fetch_v();
+  }
+  load();
+  for (; k0 < k_hi; k0 += stride) {
+    const int next = k0 + stride;
+    PG_AWAIT(NI);  // K is there (V may be in flight)
+    attend_step<F16, D, RB, KS / 16>(mine, mine + HALF, k_hi - k0, A.scale_log2, 0.f, lane >> 4, ka, va, qf, m, l, o, [&] {
+      PG_READ();  // (K is in registers)
+      if (next < k_hi) {
+        find(next);
+        fetch_k();
+        PG_AWAIT(NI);  // V is there (the next K may be in flight)
+      } else {
+        PG_AWAIT(0);
+      }
+    });
+    PG_READ();
+    if (next < k_hi) fetch_v();
+  }
+  return pages.bad;
+}
+
+template <int RB, int N>
+__device__ __forceinline__ void clear(float (&m)[RB], f32x4 (&l)[RB], f32x4 (&o)[RB][N]) {
+#pragma unroll
+  for (int rb = 0; rb < RB; rb++) {
+    m[rb] = -INFINITY;
+    l[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int dt = 0; dt < N; dt++) o[rb][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+}
+
+// The keys of one run for up to 16 query rows, by one wave.
+template <bool F16, int D>
+__device__ __forceinline__ void wave_part(const AttnArgs& A, const Run& run, int h, int b, int row0, int rows, int slot, bool only,
+                                          uint32_t mine, int lane) {
+  const Lanes<D, false> lk(lane);
+  const Lanes<D, true> lv(lane);
+  u32x4 qf[1][D / 32];
+  float m[1];
+  f32x4 l[1], o[1][D / 16];
+  clear(m, l, o);
+  const bool bad = walk<F16, D, 1>(A, run, h, run.lo, KS, mine, lane, lk, lv, qf, m, l, o,
+                                   [&] { load_q<D, 1>(A, h, b, row0, rows, lane & 15, lane >> 4, qf); });
+  const int r = row0 + (lane & 15);
+  if (r < rows)
+#pragma unroll
+    for (int dt = 0; dt < D / 16; dt++)
+      store_o<F16, D, false>(A, slot, only, h, b, r, 16 * dt + 4 * (lane >> 4), o[0][dt], m[0], bad ? NAN : l[0][0]);
+}
+
+// The keys of N runs for up to RB * 16 query rows, by a workgroup: its waves take steps in turn and do not wait for each
+// other until the end.
 template <bool F16, int D, int RB, int N, bool DEV>
 __device__ __forceinline__ void own_part(const AttnArgs& A, const Run (&runs)[N], int h, int b0, int row0, int rows, int slot,
                                          bool only, uint32_t lds, float (*s_m)[64], float (*s_l)[64]) {
-  constexpr uint32_t HALF = KS * D * 2, WAVE = 2 * HALF;  // bytes of a step's K (or V), and of a wave
-  constexpr int NI = KS * D * 2 / 1024;                   // DMA instructions of a step's K (or V)
+  constexpr uint32_t WAVE = 2 * KS * D * 2;  // bytes of a wave
   static_assert(RB * 16 * D * 4 <= (int)WAVE, "a wave's output fits its LDS");
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, kg = lane >> 4;
   const uint32_t mine = lds + WAVE * wv;
@@ -535,63 +619,13 @@ __device__ __forceinline__ void own_part(const AttnArgs& A, const Run (&runs)[N]
   u32x4 qf[RB][D / 32];
   float m[RB];
   f32x4 l[RB], o[RB][D / 16];
-#pragma unroll
-  for (int rb = 0; rb < RB; rb++) {
-    m[rb] = -INFINITY;
-    l[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int dt = 0; dt < D / 16; dt++) o[rb][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  const uint32_t ka = k_frag<D>(r16, kg), va = v_frag<D>(r16, kg);
+  clear(m, l, o);
   bool bad = false;
 #pragma unroll
-  for (int n = 0; n < N; n++) {
-    const int k_hi = runs[n].hi;
-    int k0 = runs[n].lo + KS * wv;
-    const bool any = k0 < k_hi;  // (the wave's)
-    Pages pages(runs[n].table, A.num_pages, runs[n].lo >> A.lp, max(runs[n].lo, k_hi - 1) >> A.lp, lane, any);
-    size_t at[2];  // a step's two tiles
-    int last[2];
-    auto find = [&](int k0) {
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        const Tile t(pages, A, h, D, k0 + 16 * i, k_hi - 1, lane);
-        at[i] = t.at;
-        last[i] = t.last;
-      }
-    };
-    auto fetch_k = [&] {
-#pragma unroll
-      for (int i = 0; i < 2; i++) lk.template fetch<true>(A.k + at[i], last[i], mine + HALF / 2 * i, lane);
-    };
-    auto fetch_v = [&] {
-#pragma unroll
-      for (int i = 0; i < 2; i++) lv.template fetch<true>(A.v + at[i], last[i], mine + HALF + HALF / 2 * i, lane);
-    };
-    if (any) {
-      find(k0);
-      fetch_k();
-      fetch_v();
-    }
-    if (n == 0) load_q<D, RB>(A, h, b0, row0, rows, r16, kg, qf);
-    for (; k0 < k_hi; k0 += KS * AW) {
-      const int next = k0 + KS * AW;
-      PG_AWAIT(NI);  // K is there (V may be in flight)
-      attend_step<F16, D, RB, KS / 16>(mine, mine + HALF, k_hi - k0, A.scale_log2, 0.f, kg, ka, va, qf, m, l, o, [&] {
-        PG_READ();  // (K is in registers)
-        if (next < k_hi) {
-          find(next);
-          fetch_k();
-          PG_AWAIT(NI);  // V is there (the next K may be in flight)
-        } else {
-          PG_AWAIT(0);
-        }
-      });
-      PG_READ();
-      if (next < k_hi) fetch_v();
-    }
-    bad |= pages.bad;
-  }
+  for (int n = 0; n < N; n++)
+    bad |= walk<F16, D, RB>(A, runs[n], h, runs[n].lo + KS * wv, KS * AW, mine, lane, lk, lv, qf, m, l, o, [&] {
+      if (n == 0) load_q<D, RB>(A, h, b0, row0, rows, r16, kg, qf);
+    });
   // ---- join the waves: each scales its output to the rows' common maximum and leaves it in its LDS (row:
   // D / 4 pieces of 16 bytes, swizzled with the row), then all add the four up
 #pragma unroll
@@ -665,13 +699,7 @@ __device__ __forceinline__ void prefix_part(const AttnArgs& A, int h, int row0, 
   load_q<D, RB>(A, h, 0, mine, rows, r16, kg, qf);
   float m[RB];
   f32x4 l[RB], o[RB][D / 16];
-#pragma unroll
-  for (int rb = 0; rb < RB; rb++) {
-    m[rb] = -INFINITY;
-    l[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int dt = 0; dt < D / 16; dt++) o[rb][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  clear(m, l, o);
   const uint32_t ka = k_frag<D>(r16, kg), va = v_frag<D>(r16, kg);
   uint32_t st = 0;
   for (int k0 = k_lo; k0 < k_hi; k0 += TS, st ^= STAGE) {
@@ -785,7 +813,7 @@ template <bool F16, int D, int FORM>
 __global__ void __launch_bounds__(64 * AW, 2) attn_kernel(AttnArgs A) {
   __shared__ __align__(1024) uint8_t s_kv[4 * TS * D * 2];
   __shared__ float s_m[AW][64], s_l[AW][64];
-  static_assert(sizeof(s_kv) == AW * 2 * KS * D * 2, "the two forms take the same LDS");
+  static_assert(sizeof(s_kv) == AW * 2 * KS * D * 2, "the forms take the same LDS");
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&s_kv[0];
   if constexpr (FORM == JOINED) {
     const int h = blockIdx.x % A.hkv, id = blockIdx.x / A.hkv, tile = id % A.own_tiles, b = id / A.own_tiles;
@@ -824,7 +852,7 @@ __global__ void __launch_bounds__(64 * AW, 2) attn_kernel(AttnArgs A) {
   } else {
     // parts of the prefix and of own rows alternate, a workgroup a CU of each, while there are both
     const bool only = A.np + A.ns == 1;
-    const int n_prefix = A.hkv * A.prefix_tiles * A.np, n_own = A.hkv * A.own_tiles * A.batch * A.ns;
+    const int n_prefix = A.hkv * A.prefix_tiles * A.np, n_own = A.hkv * A.own_tiles * A.groups * A.ns;
     const int runs = min(n_prefix, n_own) / NUM_CUS, bid = blockIdx.x, run = bid / NUM_CUS, rest = bid - runs * NUM_CUS;
     const bool prefix = run < 2 * runs ? run % 2 == 0 : rest < n_prefix;
     int id = run < 2 * runs ? run / 2 * NUM_CUS + bid % NUM_CUS : rest < n_prefix ? rest : bid - n_prefix;
@@ -843,6 +871,14 @@ __global__ void __launch_bounds__(64 * AW, 2) attn_kernel(AttnArgs A) {
     }
     const int tile = id % A.own_tiles;
     id /= A.own_tiles;
+    if (A.groups < A.batch) {
+      const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), b = AW * id + wv;
+      if (b >= A.batch) return;
+      const int len = own_rows(A.lens, b, A.len_add, A.width, A.lp);
+      const Run mine = {A.tables + (size_t)b * A.t_sb + (size_t)h * A.t_sh, 0, len};
+      wave_part<F16, D>(A, mine, h, b, 16 * tile, A.g, A.np, only, lds + 4 * KS * D * wv, lane);
+      return;
+    }
     const int b = id % A.batch, part = id / A.batch;
     const int len = own_rows(A.lens, b, A.len_add, A.width, A.lp);
     const int ch = part_keys(len, A.ns), lo = part * ch, hi = min(len, lo + ch);
@@ -1195,6 +1231,10 @@ int append_rows(const AppendArgs& A, bool f16, hipStream_t stream) {
 // sequences 9.3 and 9.1), past them one workgroup's walk is the longer one (1000 keys 8.1 and 12.7), and a
 // launch costs the host 3 us (that call 17.4 us, 14.1 in one launch).
 constexpr int JOINED_KEYS = 640;
+// Own rows of more than 512 (sequence, kv head)s do not fit the chip at once as a workgroup each: short ones, up to 256
+// keys, then take a wave each, which also saves joining four (256 sequences with up to 30 own rows 7.2 us against 15.9,
+// behind 1984 rows 25.9 against 31.2; up to 200 rows 36.4 and 40.2; up to 400 55.5 against 52.1, so no more).
+constexpr int PACK_KEYS = 256, PACK_OVER = 512;
 AttnPlan plan_attention(int batch, int hkv, int g, int d, int prefix_len, int max_len) {
   AttnPlan p{};
   constexpr int WANT = 512;
@@ -1204,6 +1244,7 @@ AttnPlan plan_attention(int batch, int hkv, int g, int d, int prefix_len, int ma
   p.own_tiles = (g + 15) / 16;
   if (prefix_len > 0 && max_len > 0 && prefix_len + max_len <= JOINED_KEYS && (long long)batch * hkv * p.own_tiles <= NUM_CUS) {
     p.form = JOINED;
+    p.groups = batch;
     p.ns = 1;
     return p;
   }
@@ -1227,7 +1268,14 @@ AttnPlan plan_attention(int batch, int hkv, int g, int d, int prefix_len, int ma
     }
     p.np = parts(prefix_len, tiles, want);
   }
-  if (max_len > 0) p.ns = parts(max_len, (long long)batch * hkv * p.own_tiles, WANT);
+  p.groups = batch;
+  const long long own = (long long)batch * hkv * p.own_tiles;
+  if (max_len > 0 && max_len <= PACK_KEYS && own > PACK_OVER) {
+    p.groups = (batch + AW - 1) / AW;
+    p.ns = 1;
+  } else if (max_len > 0) {
+    p.ns = parts(max_len, own, WANT);
+  }
   const size_t rows_all = p.np + p.ns == 1 ? 0 : (size_t)(p.np + p.ns) * batch * hkv * g;
   p.out_bytes = (rows_all * d * 4 + 255) / 256 * 256;
   p.bytes = p.out_bytes + (rows_all * 8 + 255) / 256 * 256;
@@ -1252,10 +1300,10 @@ static void attn_launch(const AttnArgs& A, int form, unsigned blocks, hipStream_
 // The launches of an attention; A without its split and partial results, which come from `p` and
 // `ws` (plan_attention's bytes).
 int run_attention(AttnArgs A, const AttnPlan& p, int d, bool f16, void* ws, hipStream_t stream) {
-  A.prefix_tiles = p.prefix_tiles; A.np = p.np; A.own_tiles = p.own_tiles; A.ns = p.ns;
+  A.prefix_tiles = p.prefix_tiles; A.np = p.np; A.own_tiles = p.own_tiles; A.ns = p.ns; A.groups = p.groups;
   A.part_o = static_cast<float*>(ws);
   A.part_ml = reinterpret_cast<float2*>(static_cast<char*>(ws) + p.out_bytes);
-  const long long blocks = (long long)A.hkv * ((long long)p.prefix_tiles * p.np + (long long)p.own_tiles * A.batch * p.ns);
+  const long long blocks = (long long)A.hkv * ((long long)p.prefix_tiles * p.np + (long long)p.own_tiles * p.groups * p.ns);
   if (blocks > 0x7fffffff) return MQ_ERR_ARG;
   if (d == 128)
     f16 ? attn_launch<true, 128>(A, p.form, (unsigned)blocks, stream) : attn_launch<false, 128>(A, p.form, (unsigned)blocks, stream);
@@ -1322,7 +1370,7 @@ int sparse_attention(const MqPagePool* P, const void* q, int64_t q_sb, int64_t q
     return MQ_ERR_ARG;
   const int most = top < width ? top : width, hkv = P->num_kv_heads, g = num_q_heads / hkv;
   AttnPlan p = plan_attention(batch, hkv, g, P->head_dim, 0, most * P->page_size);
-  p.form = OWN;
+  if (p.groups == batch) p.form = OWN;  // (else there is one part)
   const size_t head = chosen_bytes(batch, hkv, g, top);
   if (!workspace_ok(ws, ws_bytes, head + p.bytes)) return MQ_ERR_ARG;
   AttnArgs A = attn_args(*P, q, q_sb, q_sh, out, o_sb, o_sh, num_q_heads, batch, scale);

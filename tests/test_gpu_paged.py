@@ -307,6 +307,60 @@ def test_shared_prefix_attention_of_large_batches(case):
     _check(out, q, rows_of, 1 / math.sqrt(d))
 
 
+@pytest.mark.parametrize("case", [
+    # more than 512 sequences times kv heads with at most 256 own rows: a wave a sequence
+    (130, 4, 2, 128, 64, BF, 0, [0, 1, 31, 32, 33, 64, 100, 256, 255, 129]),
+    (130, 4, 2, 128, 64, BF, 70, [0, 1, 31, 32, 33, 64, 100, 256, 255, 129]),
+    (65, 8, 17, 64, 16, FP, 300, [0, 16, 17, 200]),
+    (515, 1, 1, 128, 32, FP, 1500, [5]),
+    (103, 5, 3, 64, 256, BF, 0, [0, 0, 7]),
+], ids=lambda c: f"b{c[0]}h{c[1]}x{c[2]}d{c[3]}p{c[4]}n{c[6]}")
+def test_shared_prefix_attention_of_many_short_sequences(case):
+    from megaqwen_amd import paged
+
+    B, hkv, G, d, page, dtype, prefix, some = case
+    lens = (some * B)[:B]
+    q, k, v, pre, tables, lens_d, rows_of = _setup(B, hkv, G, d, page, dtype, prefix, lens, seed=B)
+    out = paged.shared_prefix_attention(q, k, v, pre, prefix, tables, lens_d, max_len=max(lens))
+    _check(out, q, rows_of, 1 / math.sqrt(d))
+    # laid out for fewer rows than there are, and (a workgroup a sequence) for more
+    for max_len in (1, 300):
+        _check(paged.shared_prefix_attention(q, k, v, pre, prefix, tables, lens_d, max_len=max_len), q, rows_of, 1 / math.sqrt(d))
+    # a page outside the pool is its own sequence's matter only
+    at = next(b for b in range(9, B) if lens[b] > 0)
+    tables[at, 0] = k.shape[0]
+    bad = paged.shared_prefix_attention(q, k, v, pre, prefix, tables, lens_d, max_len=max(lens))
+    assert bool(bad[at].isnan().all())
+    others = [b for b in range(B) if b != at]
+    assert torch.equal(_bits(bad[others]), _bits(out[others]))
+
+
+def test_sparse_attention_of_many_short_choices():
+    """More than 512 sequences times kv heads, of which each reads at most 256 rows."""
+    from megaqwen_amd import paged
+
+    B, hkv, G, d, page, top = 140, 4, 2, 64, 32, 8
+    lens = ([0, 1, 256, 255, 900, 1000, 33] * B)[:B]
+    q, k, v, _, tables, lens_d, _ = _setup(B, hkv, G, d, page, BF, 0, lens, seed=8)
+    bounds = torch.zeros(k.shape[0], hkv, 2, d, dtype=BF, device=DEV)
+    host = tables.cpu().long()
+    for b, n in enumerate(lens):
+        for i in range(-(-n // page)):
+            bounds[host[b, i]] = _key_bounds(k[host[b, i], :, : min(page, n - i * page)])
+    out, chosen = paged.sparse_attention(q, k, v, bounds, tables, lens_d, top)
+    want = {(b, j): _plain_choice(q[b, j * G:(j + 1) * G], bounds[:, j], host[b], lens[b], page, top) for b in range(B) for j in range(hkv)}
+    for (b, j), sel in want.items():
+        assert chosen[b, j].tolist() == sel + [-1] * (top - len(sel))
+
+    def rows_of(b, j):
+        sel = want[b, j]
+        n = 0 if not sel else (len(sel) - 1) * page + (lens[b] - 1) % page + 1
+        return tuple(_rows_of(t, host[b][sel], j, n) for t in (k, v))
+
+    rows_of.hkv = hkv
+    _check(out, q, rows_of, 1 / math.sqrt(d))
+
+
 def test_shared_prefix_attention_strides_scale_and_out():
     """q and out as slices of wider rows, tables as a slice of whole tables, another scale; repeats are bit-identical."""
     from megaqwen_amd import paged
