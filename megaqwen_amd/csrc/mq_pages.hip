@@ -518,14 +518,14 @@ struct Run {
   int lo, hi;
 };
 
-// The 32-key steps of a run from key k0 on, every `stride` keys, by one wave with 16 KB of LDS, half for K and half for
-// V: it asks for the next step's K as soon as it has the scores of this one, for its V once this one's is multiplied.
+// The 32-key steps of a run from key k0 on, every `stride` keys, for 16 query rows, by one wave with 16 KB of LDS, half
+// for K and half for V: it asks for the next step's K as soon as it has the scores of this one, for its V once this one's is multiplied.
 // load() brings the query fragments. The rows are read once (or, of several runs, by few workgroups), past the caches:
 // non-temporal, 6.1 against 5.4 TB/s. True if a page was outside the pool.
-template <bool F16, int D, int RB, class Load>
+template <bool F16, int D, class Load>
 __device__ __forceinline__ bool walk(const AttnArgs& A, const Run& run, int h, int k0, int stride, uint32_t mine, int lane,
-                                     const Lanes<D, false>& lk, const Lanes<D, true>& lv, u32x4 (&qf)[RB][D / 32],
-                                     float (&m)[RB], f32x4 (&l)[RB], f32x4 (&o)[RB][D / 16], Load load) {
+                                     const Lanes<D, false>& lk, const Lanes<D, true>& lv, u32x4 (&qf)[1][D / 32],
+                                     float (&m)[1], f32x4 (&l)[1], f32x4 (&o)[1][D / 16], Load load) {
   constexpr uint32_t HALF = KS * D * 2;  // bytes of a step's K (or V)
   constexpr int NI = KS * D * 2 / 1024;  // DMA instructions of it
   const uint32_t ka = k_frag<D>(lane & 15, lane >> 4), va = v_frag<D>(lane & 15, lane >> 4);
@@ -559,7 +559,7 @@ __device__ __forceinline__ bool walk(const AttnArgs& A, const Run& run, int h, i
   for (; k0 < k_hi; k0 += stride) {
     const int next = k0 + stride;
     PG_AWAIT(NI);  // K is there (V may be in flight)
-    attend_step<F16, D, RB, KS / 16>(mine, mine + HALF, k_hi - k0, A.scale_log2, 0.f, lane >> 4, ka, va, qf, m, l, o, [&] {
+    attend_step<F16, D, 1, KS / 16>(mine, mine + HALF, k_hi - k0, A.scale_log2, 0.f, lane >> 4, ka, va, qf, m, l, o, [&] {
       PG_READ();  // (K is in registers)
       if (next < k_hi) {
         find(next);
@@ -596,7 +596,7 @@ __device__ __forceinline__ void wave_part(const AttnArgs& A, const Run& run, int
   float m[1];
   f32x4 l[1], o[1][D / 16];
   clear(m, l, o);
-  const bool bad = walk<F16, D, 1>(A, run, h, run.lo, KS, mine, lane, lk, lv, qf, m, l, o,
+  const bool bad = walk<F16, D>(A, run, h, run.lo, KS, mine, lane, lk, lv, qf, m, l, o,
                                    [&] { load_q<D, 1>(A, h, b, row0, rows, lane & 15, lane >> 4, qf); });
   const int r = row0 + (lane & 15);
   if (r < rows)
@@ -605,60 +605,53 @@ __device__ __forceinline__ void wave_part(const AttnArgs& A, const Run& run, int
       store_o<F16, D, false>(A, slot, only, h, b, r, 16 * dt + 4 * (lane >> 4), o[0][dt], m[0], bad ? NAN : l[0][0]);
 }
 
-// The keys of N runs for up to RB * 16 query rows, by a workgroup: its waves take steps in turn and do not wait for each
+// The keys of N runs for up to 16 query rows, by a workgroup: its waves take steps in turn and do not wait for each
 // other until the end.
-template <bool F16, int D, int RB, int N, bool DEV>
+template <bool F16, int D, int N, bool DEV>
 __device__ __forceinline__ void own_part(const AttnArgs& A, const Run (&runs)[N], int h, int b0, int row0, int rows, int slot,
-                                         bool only, uint32_t lds, float (*s_m)[64], float (*s_l)[64]) {
+                                         bool only, uint32_t lds, float (*s_m)[16], float (*s_l)[16]) {
   constexpr uint32_t WAVE = 2 * KS * D * 2;  // bytes of a wave
-  static_assert(RB * 16 * D * 4 <= (int)WAVE, "a wave's output fits its LDS");
+  static_assert(16 * D * 4 <= (int)WAVE, "a wave's output fits its LDS");
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, kg = lane >> 4;
   const uint32_t mine = lds + WAVE * wv;
   const Lanes<D, false> lk(lane);
   const Lanes<D, true> lv(lane);
-  u32x4 qf[RB][D / 32];
-  float m[RB];
-  f32x4 l[RB], o[RB][D / 16];
+  u32x4 qf[1][D / 32];
+  float m[1];
+  f32x4 l[1], o[1][D / 16];
   clear(m, l, o);
   bool bad = false;
 #pragma unroll
   for (int n = 0; n < N; n++)
-    bad |= walk<F16, D, RB>(A, runs[n], h, runs[n].lo + KS * wv, KS * AW, mine, lane, lk, lv, qf, m, l, o, [&] {
-      if (n == 0) load_q<D, RB>(A, h, b0, row0, rows, r16, kg, qf);
+    bad |= walk<F16, D>(A, runs[n], h, runs[n].lo + KS * wv, KS * AW, mine, lane, lk, lv, qf, m, l, o, [&] {
+      if (n == 0) load_q<D, 1>(A, h, b0, row0, rows, r16, kg, qf);
     });
   // ---- join the waves: each scales its output to the rows' common maximum and leaves it in its LDS (row:
   // D / 4 pieces of 16 bytes, swizzled with the row), then all add the four up
-#pragma unroll
-  for (int rb = 0; rb < RB; rb++) {
-    if (kg == 0) {
-      s_m[wv][16 * rb + r16] = m[rb];
-      s_l[wv][16 * rb + r16] = bad ? NAN : l[rb][0];
-    }
+  if (kg == 0) {
+    s_m[wv][r16] = m[0];
+    s_l[wv][r16] = bad ? NAN : l[0][0];
   }
   __syncthreads();
+  float top = s_m[0][r16];
 #pragma unroll
-  for (int rb = 0; rb < RB; rb++) {
-    const int r = 16 * rb + r16;
-    float mx = s_m[0][r];
+  for (int w = 1; w < AW; w++) top = fmaxf(top, s_m[w][r16]);
+  const float f = m[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[0] - top);
 #pragma unroll
-    for (int w = 1; w < AW; w++) mx = fmaxf(mx, s_m[w][r]);
-    const float f = m[rb] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rb] - mx);
+  for (int dt = 0; dt < D / 16; dt++) {
+    f32x4 x = o[0][dt];
 #pragma unroll
-    for (int dt = 0; dt < D / 16; dt++) {
-      f32x4 x = o[rb][dt];
-#pragma unroll
-      for (int e = 0; e < 4; e++) x[e] *= f;
-      *(lds_f32x4*)(uintptr_t)(mine + r * (4 * D) + 16 * ((4 * dt + kg) ^ r16)) = x;
-    }
+    for (int e = 0; e < 4; e++) x[e] *= f;
+    *(lds_f32x4*)(uintptr_t)(mine + r16 * (4 * D) + 16 * ((4 * dt + kg) ^ r16)) = x;
   }
   __syncthreads();
   constexpr int PPR = D / 4;  // 16-byte pieces a row
-  const int n = min(RB * 16, rows - row0) * PPR;
+  const int n = min(16, rows - row0) * PPR;
   for (int i = tid; i < n; i += 64 * AW) {
     const int r = i / PPR, p = i % PPR;
     f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < AW; w++) x += *(lds_f32x4*)(uintptr_t)(lds + WAVE * w + r * (4 * D) + 16 * (p ^ (r & 15)));
+    for (int w = 0; w < AW; w++) x += *(lds_f32x4*)(uintptr_t)(lds + WAVE * w + r * (4 * D) + 16 * (p ^ r));
     float mx = s_m[0][r], sum = 0.f;
 #pragma unroll
     for (int w = 1; w < AW; w++) mx = fmaxf(mx, s_m[w][r]);
@@ -729,13 +722,14 @@ __device__ __forceinline__ int own_rows(const int* lens, int b, int add, int wid
 constexpr int UNIT = KS * AW;
 __host__ __device__ __forceinline__ int part_keys(int len, int parts) { return ((len + parts - 1) / parts + UNIT - 1) / UNIT * UNIT; }
 
-// How the query rows of a prefix are tiled: up to 32 rows, all keys' work is split among the waves (own_part);
-// more rows are (prefix_part). JOINED: no tiles of the prefix; each sequence's workgroup goes over the prefix and
-// then over its own rows, so that nothing is left to join and the call is one launch. OWN: no prefix, and the last
-// workgroup of a sequence's parts joins them (a launch before has cleared the tickets that tell which one is last): the
-// GPU's time is that of a second launch (one sequence over 64 of 250 pages 15.8 us, 16.0 with it), the host's 4 us less.
-enum : int { ROWS16 = 0, ROWS32 = 1, ROWS64 = 2, ROWS128 = 3, JOINED = 4, OWN = 5 };
-__host__ __device__ constexpr int tile_rows(int form) { return 16 << form; }
+// How the query rows of a prefix are tiled: for up to 16 rows, the keys are split among the waves (own_part); of more,
+// the rows are (prefix_part; 32 rows behind 8192 14.8 us, 21.4 with the keys split). JOINED: no tiles of the prefix; each
+// sequence's workgroup goes over the prefix and then over its own rows, so that nothing is left to join and the call is
+// one launch. OWN: no prefix, and the last workgroup of a sequence's parts joins them (a launch before has cleared the
+// tickets that tell which one is last): the GPU's time is that of a second launch (one sequence over 64 of 250 pages
+// 15.8 us, 16.0 with it), the host's 4 us less.
+enum : int { ROWS16, ROWS64, ROWS128, JOINED, OWN };
+__host__ __device__ constexpr int tile_rows(int form) { return form == ROWS16 ? 16 : form == ROWS64 ? 64 : 128; }
 
 // One row (query head, sequence), by one wave: the parts' outputs, scaled to their common maximum, over their sums. Rows
 // without a key give zeros. Lane p takes part p's maximum and sum (and part p + 64's); LPR lanes hold
@@ -812,14 +806,14 @@ __device__ __forceinline__ void join_row(const AttnArgs& A, size_t row, int part
 template <bool F16, int D, int FORM>
 __global__ void __launch_bounds__(64 * AW, 2) attn_kernel(AttnArgs A) {
   __shared__ __align__(1024) uint8_t s_kv[4 * TS * D * 2];
-  __shared__ float s_m[AW][64], s_l[AW][64];
+  __shared__ float s_m[AW][16], s_l[AW][16];
   static_assert(sizeof(s_kv) == AW * 2 * KS * D * 2, "the forms take the same LDS");
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&s_kv[0];
   if constexpr (FORM == JOINED) {
     const int h = blockIdx.x % A.hkv, id = blockIdx.x / A.hkv, tile = id % A.own_tiles, b = id / A.own_tiles;
     const int len = own_rows(A.lens, b, A.len_add, A.width, A.lp);
     const Run runs[2] = {{A.prefix_pages, 0, A.prefix_len}, {A.tables + (size_t)b * A.t_sb + (size_t)h * A.t_sh, 0, len}};
-    own_part<F16, D, 1, 2, false>(A, runs, h, b, 16 * tile, A.g, 0, true, lds, s_m, s_l);
+    own_part<F16, D, 2, false>(A, runs, h, b, 16 * tile, A.g, 0, true, lds, s_m, s_l);
   } else if constexpr (FORM == OWN) {
     int id = blockIdx.x;
     const int h = id % A.hkv;
@@ -837,7 +831,7 @@ __global__ void __launch_bounds__(64 * AW, 2) attn_kernel(AttnArgs A) {
     }
     const int parts = (len + ch - 1) / ch;
     const Run mine[1] = {{A.tables + (size_t)b * A.t_sb + (size_t)h * A.t_sh, lo, hi}};
-    own_part<F16, D, 1, 1, true>(A, mine, h, b, 16 * tile, A.g, part, parts == 1, lds, s_m, s_l);
+    own_part<F16, D, 1, true>(A, mine, h, b, 16 * tile, A.g, part, parts == 1, lds, s_m, s_l);
     if (parts == 1) return;
     PG_AWAIT(0);  // the wave's stores have been written, and after the barrier every wave's
     __shared__ int s_last;
@@ -861,9 +855,9 @@ __global__ void __launch_bounds__(64 * AW, 2) attn_kernel(AttnArgs A) {
     if (prefix) {
       const int rows = A.batch * A.g, row0 = tile_rows(FORM) * (id % A.prefix_tiles), part = id / A.prefix_tiles;
       const int ch = part_keys(A.prefix_len, A.np), lo = part * ch, hi = min(A.prefix_len, lo + ch);
-      if constexpr (FORM <= ROWS32) {
+      if constexpr (FORM == ROWS16) {
         const Run mine[1] = {{A.prefix_pages, lo, hi}};
-        own_part<F16, D, FORM == ROWS16 ? 1 : 2, 1, false>(A, mine, h, 0, row0, rows, part, only, lds, s_m, s_l);
+        own_part<F16, D, 1, false>(A, mine, h, 0, row0, rows, part, only, lds, s_m, s_l);
       } else {
         prefix_part<F16, D, FORM == ROWS64 ? 1 : 2>(A, h, row0, rows, lo, hi, part, only, lds);
       }
@@ -892,7 +886,7 @@ __global__ void __launch_bounds__(64 * AW, 2) attn_kernel(AttnArgs A) {
       return;
     }
     const Run mine[1] = {{A.tables + (size_t)b * A.t_sb + (size_t)h * A.t_sh, lo, hi}};
-    own_part<F16, D, 1, 1, false>(A, mine, h, b, 16 * tile, A.g, A.np + part, only, lds, s_m, s_l);
+    own_part<F16, D, 1, false>(A, mine, h, b, 16 * tile, A.g, A.np + part, only, lds, s_m, s_l);
   }
 }
 
@@ -1217,14 +1211,17 @@ int append_rows(const AppendArgs& A, bool f16, hipStream_t stream) {
 // 2000 rows with up to 64 own 14.5 us against 17.7, 23 behind 1117 with 5 queries a kv head 8.2 against 9.5; the other
 // way from some 2000 steps on: 128 behind 8192 with up to 500 own 40.8 against 45.8 with tiles of 64, 256 behind 15001
 // with up to 1024 110 against 130). A sequence's own rows are shared by its G query heads a kv head only, in
-// tiles of 16. Keys are split until the launch has about two workgroups a CU, in parts of at least 128 keys.
-// Each part's result is another 4 D + 8 bytes a query row written and read, so tiles of more than 32 rows take fewer
-// parts where those cost nothing (us a captured call):
-// - beside own rows as many as end about when these do, at 1.8 us for 64 keys of a tile and 5.4 TB/s for half of the
-//   longest own length a sequence (64 sequences behind 8192 rows with up to 2000 own: 60 against 74 with no such limit;
-//   256 behind 15001 with up to 1024: 113 against 138; at 1.45 us, an alone tile's time, 68 and 120);
+// tiles of 16. Keys are split until the launch has about two workgroups a CU, in parts of at least 128 keys, of 256 where
+// there would be more than 32 (one sequence with 8192 own rows 12.3 us in 32 parts, 13.7 in 64; with 30000 15.9 in 64 and
+// 17.9 in 32, at two kv heads).
+// Each part's result is another 4 D + 8 bytes a query row written and read, so a prefix takes fewer parts where those
+// cost nothing (us a captured call):
+// - tiles of more than 16 rows beside own rows as many as end about when these do, at 1.8 us for 64 keys of a tile and
+//   5.4 TB/s for half of the longest own length a sequence (64 sequences behind 8192 rows with up to 2000 own: 60 against
+//   74 with no such limit; 256 behind 15001 with up to 1024: 113 against 138; at 1.45 us, an alone tile's time, 68 and 120);
 // - of a prefix of few steps, at most 16 each, 192 workgroups, since what a part costs before and after its steps is
-//   several of them (64 behind 8192 with up to 200 own: 24 against 28; 20 behind 15000 with up to 500: 22 against 26).
+//   several of them (64 behind 8192 with up to 200 own: 24 against 28; 20 behind 15000 with up to 500: 22 against 26), and
+//   so for tiles of 16 rows at any length (8 sequences behind 8192 13.5 against 18.3, behind 30000 26.8 against 28.3).
 //
 // Short contexts of few sequences take one launch instead (JOINED), whose workgroups go over prefix and own rows alike:
 // up to 640 keys the two cost the GPU the same (4 sequences behind 512 rows 7.3 us in two launches, 7.6 in one; 32
@@ -1237,7 +1234,7 @@ constexpr int JOINED_KEYS = 640;
 constexpr int PACK_KEYS = 256, PACK_OVER = 512;
 AttnPlan plan_attention(int batch, int hkv, int g, int d, int prefix_len, int max_len) {
   AttnPlan p{};
-  constexpr int WANT = 512;
+  constexpr int WANT = 512, MANY = 32;
   constexpr long long HALF_TILES = 1024;
   constexpr double STEP_US = 1.8, SHORT_WANT = 192., SHORT_STEPS = 16.;
   const int rows = batch * g;
@@ -1249,9 +1246,9 @@ AttnPlan plan_attention(int batch, int hkv, int g, int d, int prefix_len, int ma
     return p;
   }
   const long long steps128 = (long long)hkv * ((rows + 127) / 128) * ((prefix_len + TS - 1) / TS);
-  p.form = rows <= 16 ? ROWS16 : rows <= 32 ? ROWS32 : rows <= 64 || steps128 <= HALF_TILES ? ROWS64 : ROWS128;
+  p.form = rows <= 16 ? ROWS16 : rows <= 64 || steps128 <= HALF_TILES ? ROWS64 : ROWS128;
   auto parts = [&](int len, long long tiles, double want) {
-    const int most = (len + UNIT - 1) / UNIT;
+    const int units = (len + UNIT - 1) / UNIT, most = units <= MANY ? units : units / 2 > MANY ? units / 2 : MANY;
     double n = ceil(want / (double)tiles);
     n = fmax(1., fmin(n, fmin(most, MAX_PARTS / 2)));
     const int ch = part_keys(len, (int)n);
@@ -1261,11 +1258,9 @@ AttnPlan plan_attention(int batch, int hkv, int g, int d, int prefix_len, int ma
     p.prefix_tiles = (rows + tile_rows(p.form) - 1) / tile_rows(p.form);
     const long long tiles = (long long)hkv * p.prefix_tiles;
     double want = WANT;
-    if (p.form >= ROWS64) {
-      const double steps = (double)tiles * ((prefix_len + TS - 1) / TS), own_us = (double)batch * hkv * max_len * d * 2 / 5.4e6;
-      if (own_us > 0.) want = fmin(want, steps * STEP_US / own_us);
-      if (steps <= SHORT_STEPS * SHORT_WANT) want = fmin(want, SHORT_WANT);
-    }
+    const double steps = (double)tiles * ((prefix_len + TS - 1) / TS), own_us = (double)batch * hkv * max_len * d * 2 / 5.4e6;
+    if (p.form != ROWS16 && own_us > 0.) want = fmin(want, steps * STEP_US / own_us);
+    if (p.form == ROWS16 || steps <= SHORT_STEPS * SHORT_WANT) want = fmin(want, SHORT_WANT);
     p.np = parts(prefix_len, tiles, want);
   }
   p.groups = batch;
@@ -1287,7 +1282,6 @@ static void attn_launch(const AttnArgs& A, int form, unsigned blocks, hipStream_
   if (blocks > 0) {
     switch (form) {
       case ROWS16: attn_kernel<F16, D, ROWS16><<<blocks, 64 * AW, 0, stream>>>(A); break;
-      case ROWS32: attn_kernel<F16, D, ROWS32><<<blocks, 64 * AW, 0, stream>>>(A); break;
       case ROWS64: attn_kernel<F16, D, ROWS64><<<blocks, 64 * AW, 0, stream>>>(A); break;
       case JOINED: attn_kernel<F16, D, JOINED><<<blocks, 64 * AW, 0, stream>>>(A); break;
       case OWN: attn_kernel<F16, D, OWN><<<blocks, 64 * AW, 0, stream>>>(A); return;
