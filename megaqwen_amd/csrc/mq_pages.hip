@@ -1232,6 +1232,9 @@ constexpr int JOINED_KEYS = 640;
 // keys, then take a wave each, which also saves joining four (256 sequences with up to 30 own rows 7.2 us against 15.9,
 // behind 1984 rows 25.9 against 31.2; up to 200 rows 36.4 and 40.2; up to 400 55.5 against 52.1, so no more).
 constexpr int PACK_KEYS = 256, PACK_OVER = 512;
+// Without a prefix, up to 512 own rows stay one part, and the call one launch: 4 sequences with up to 200 rows 6.0 us
+// against 7.6 in two parts, 400 rows 7.9 and 7.7, 600 9.4 and 7.9; 40 with up to 400 11.7 and 14.1.
+constexpr int WHOLE_KEYS = 512;
 AttnPlan plan_attention(int batch, int hkv, int g, int d, int prefix_len, int max_len) {
   AttnPlan p{};
   constexpr int WANT = 512, MANY = 32;
@@ -1269,7 +1272,7 @@ AttnPlan plan_attention(int batch, int hkv, int g, int d, int prefix_len, int ma
     p.groups = (batch + AW - 1) / AW;
     p.ns = 1;
   } else if (max_len > 0) {
-    p.ns = parts(max_len, own, WANT);
+    p.ns = prefix_len == 0 && max_len <= WHOLE_KEYS ? 1 : parts(max_len, own, WANT);
   }
   const size_t rows_all = p.np + p.ns == 1 ? 0 : (size_t)(p.np + p.ns) * batch * hkv * g;
   p.out_bytes = (rows_all * d * 4 + 255) / 256 * 256;

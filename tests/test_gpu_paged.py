@@ -517,7 +517,7 @@ def test_sparse_parts_join_in_a_replayed_graph(G, d):
     """Sequences of no, one and many parts, whose lengths change between the replays of one graph; all pages are chosen."""
     from megaqwen_amd import paged
 
-    hkv, page, top = 2, 64, 48
+    hkv, page, top = 2, 64, 47
     lens = [3000, 128, 129, 1500, 3000, 1]
     q, k, v, _, tables, lens_d, rows_of = _setup(6, hkv, G, d, page, BF, 0, lens, seed=G)
     bounds = torch.zeros(k.shape[0], hkv, 2, d, dtype=BF, device=DEV)  # (never decides: no sequence has more pages)
